@@ -308,7 +308,7 @@ def _plain_append(s):
         x = x.float()
         a = torch.where(x.isfinite(), x.abs(), 0).amax(-1)
         m, e = torch.frexp(a)  # a = m 2^e with m in [1/2, 1); 448 = (7/8) 2^9
-        e = (e - 9 + (m > 0.875).int()).clamp(-126, 127)
+        e = torch.where(a > 0, e - 9 + (m > 0.875).int(), -126).clamp(-126, 127)  # the least e with a <= 448 2^e
         codes = (x * torch.exp2(-e.double()).float()[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn)
         pool[page, :, off] = codes.view(torch.uint8)
         scales[page, :, off] = (e + 127).to(torch.uint8)
