@@ -47,7 +47,8 @@ typedef enum {
   MPC_ERR_COMPILE = 9      /* NVRTC unavailable or it could not compile a fused expression */
 } mpc_status;
 
-typedef enum { MPC_F32 = 0, MPC_F16 = 1, MPC_BF16 = 2, MPC_I32 = 3, MPC_BOOL = 4 } mpc_dtype;
+typedef enum { MPC_F32 = 0, MPC_F16 = 1, MPC_BF16 = 2, MPC_I32 = 3, MPC_BOOL = 4,
+               MPC_E4M3 = 5 /* paged caches only */ } mpc_dtype;
 
 typedef struct mpc_device mpc_device; /* one per CUDA device ordinal and process */
 typedef void *mpc_stream;             /* a cudaStream_t; NULL = the device's own stream */
@@ -303,6 +304,89 @@ int mpc_geglu(mpc_device *dev, const void *x, int32_t dtype, void *out, int64_t 
  * nn-kernels.ts:256-271). */
 int mpc_mean_pool(mpc_device *dev, const void *x, int32_t dtype, const void *mask, int32_t mask_dtype, void *out,
                   int64_t B, int64_t L, int64_t D, mpc_stream s);
+
+/* ---- the paged key/value cache (no reference counterpart: MultiheadAttention recomputes K and V of
+ * the whole sequence, packages/tensor-autograd/src/transformer.ts:173-242) ---------------------------
+ * K pages [n_pages, hk, page_size, d] and V pages [n_pages, hk, page_size, dv], contiguous. A block table
+ * i32 [n_seq, max_pages] names each sequence's pages in order: its position p lives in page
+ * table[seq, p / page_size], row p % page_size. Several sequences may share a page they only read.
+ * dtype MPC_F32 / F16 / BF16 stores the rows as they are; MPC_E4M3 stores each row in 8 bits with one
+ * scale byte per (page, head, row) in k_scale / v_scale [n_pages, hk, page_size]: the row's value is
+ * code * 2^(byte - 127), the byte the least one whose scaled row stays within 448 (infinities saturate,
+ * NaN stays). Head dims up to 256. A token whose sequence, position or page lies outside the cache is
+ * left out by the kernel, and the next synchronisation returns MPC_ERR_INVALID naming it (once). */
+typedef struct {
+  int64_t n_pages, page_size, hk, d, dv;
+  int32_t dtype; /* MPC_F32, MPC_F16, MPC_BF16 or MPC_E4M3 */
+  int32_t reserved;
+} mpc_kv_desc;
+/* n tokens' dense rows: K element (t, head, i) at t * k_stride[0] + head * k_stride[1] + i, V likewise, so a
+ * packed projection is read in place. dtype f32, f16 or bf16. */
+typedef struct {
+  int64_t n, n_seq, max_pages; /* the table is [n_seq, max_pages] */
+  int64_t k_stride[2], v_stride[2];
+  int32_t dtype;
+  int32_t reserved;
+} mpc_kv_tokens;
+/* Writes token t's K and V rows at position pos[t] of sequence seq[t] (seq NULL: sequence t). pos[t] < 0
+ * is padding: nothing is written. The rows' dtype is the cache's, or any float type into MPC_E4M3. Two
+ * tokens of one call must not name the same place: which of their bytes stay is not defined. */
+int mpc_kv_append(mpc_device *dev, const mpc_kv_desc *cache, void *k_pages, void *v_pages, uint8_t *k_scale,
+                  uint8_t *v_scale, const mpc_kv_tokens *tokens, const void *k, const void *v, const int32_t *table,
+                  const int32_t *seq, const int32_t *pos, mpc_stream s);
+/* Reads the rows at (seq[t], pos[t]) into dense K / V of any float dtype (one rounding); a padding token's
+ * or a bad token's rows are zeros. */
+int mpc_kv_read(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, const void *v_pages,
+                const uint8_t *k_scale, const uint8_t *v_scale, const mpc_kv_tokens *tokens, void *k, void *v,
+                const int32_t *table, const int32_t *seq, const int32_t *pos, mpc_stream s);
+
+/* Attention of one new token per sequence over the paged cache: for sequence i and head h,
+ * O[i,h] = softmax_j(scale * Q[i,h] . K[j, h / (h / hk)]) V over positions j < lengths[i] (the new token's own
+ * row included, once appended). Heads share K/V in groups of h / hk. A length of 0 gives zeros and
+ * LSE -inf; rows behind a sequence's length are never used, whatever they hold. Q [b, h, d] and O
+ * [b, h, dv] have element strides (sequence, head) and a contiguous last axis; their dtype is the cache's,
+ * or any float type over MPC_E4M3. LSE (optional, f32 [b, h]) is the natural-log normaliser. The work is
+ * split along the cache by the lengths found on the device and joined by a second small kernel; the
+ * partial results live in the workspace. A length that is negative or beyond max_pages * page_size, or a
+ * page outside the cache, is cut off or left out, and the next synchronisation returns MPC_ERR_INVALID. */
+typedef struct {
+  int64_t b, h, max_pages;
+  int64_t q_stride[2], o_stride[2];
+  int32_t dtype; /* of Q and O */
+  float scale;
+} mpc_sdpa_paged_desc;
+/* Bytes that mpc_sdpa_paged needs as workspace for any lengths within the table. */
+int mpc_sdpa_paged_workspace(mpc_device *dev, const mpc_kv_desc *cache, const mpc_sdpa_paged_desc *desc, size_t *bytes);
+/* workspace NULL: taken from the device's allocator for this call (not while s is being captured into a
+ * graph). A workspace given must not be used by another call at the same time; graphs that may run side
+ * by side need one each. 16-byte aligned. */
+int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, const void *v_pages,
+                   const uint8_t *k_scale, const uint8_t *v_scale, const mpc_sdpa_paged_desc *desc, const void *Q,
+                   const int32_t *table, const int32_t *lengths, void *O, float *LSE, void *workspace,
+                   size_t workspace_bytes, mpc_stream s);
+
+/* ---- sampling: the next token of each row of logits from one uniform number per row -----------------
+ * With w_i = exp((logit_i - max) / temperature) and the tokens ranked by logit (ties: the lowest index
+ * first), the kept set is the first top_k ranks, of those the ranks before which less than top_p of the
+ * top-k's weight lies, of those the ones with w_i >= min_p; the first rank is always kept. The token is
+ * the lowest index at which the kept weights' running sum exceeds u times their total. Weights are
+ * evaluated in f64 and summed as integers (2^-46 of the largest weight at 2^16 tokens), so the result
+ * does not depend on the order of the sum.
+ * temperature <= 0 (or NaN): the largest logit, lowest index first. top_k <= 0, top_p >= 1, min_p <= 0: off.
+ * NaN logits count as -inf; a row with nothing above -inf gives token -1, prob 0, kept 0. u is clamped
+ * to [0, 1) (NaN: 0). */
+typedef struct {
+  int64_t rows, vocab, row_stride; /* logits element (r, i) at r * row_stride + i */
+  int32_t dtype;                   /* MPC_F32, MPC_F16 or MPC_BF16 */
+  int32_t top_k;                   /* the settings of every row, where the per-row array is NULL */
+  float temperature, top_p, min_p;
+  int32_t reserved;
+} mpc_sample_desc;
+/* prob (optional, f32 [rows]): the token's share of the kept weight; kept (optional, i32 [rows]): the size
+ * of the kept set. The per-row settings are device arrays or NULL. */
+int mpc_sample(mpc_device *dev, const mpc_sample_desc *desc, const void *logits, const float *u,
+               const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, int32_t *token,
+               float *prob, int32_t *kept, mpc_stream s);
 
 /* ---- element-wise fusion (WebGpuDevice.fuse / compile, packages/tensor-webgpu/src/facade.ts:137-164,
  * lowering as fusion-wgsl.ts:303-431) ------------------------------------------------------------

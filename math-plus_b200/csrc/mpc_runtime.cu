@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "kv_cache.cuh"
 #include "mpc_internal.h"
 #include "sm100.cuh"
 
@@ -431,12 +432,26 @@ int mpc_device_stream(mpc_device *dev, mpc_stream *s) {
 }
 
 static int read_error_word(mpc_device *dev) {
-  int word = 0;
-  cudaError_t e = cudaMemcpy(&word, dev->d_err, sizeof(int), cudaMemcpyDeviceToHost);
+  int word[3] = {0, 0, 0};
+  cudaError_t e = cudaMemcpy(word, dev->d_err, sizeof(word), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(dev, e, "reading the kernel error word");
-  if (word) {
+  if (word[0]) {
     dev->sticky = MPC_ERR_TIMEOUT;
-    return fail(MPC_ERR_TIMEOUT, "a kernel's bounded wait ran out (site 0x%x); its results are invalid", word);
+    return fail(MPC_ERR_TIMEOUT, "a kernel's bounded wait ran out (site 0x%x); its results are invalid", word[0]);
+  }
+  if (word[1]) {  // the kernel left the access out and went on, so the handle stays usable: report once
+    MPC_CUDA(dev, cudaMemset(dev->d_err + 1, 0, 2 * sizeof(int)));
+    switch (word[1]) {
+      case kBadAppendRead:
+        return fail(MPC_ERR_INVALID, "paged cache: token %d names a sequence, position or page outside the cache",
+                    word[2]);
+      case kBadAttend:
+        return fail(MPC_ERR_INVALID, "paged cache: the block table of sequence %d names a page outside the cache",
+                    word[2]);
+      default:
+        return fail(MPC_ERR_INVALID, "paged cache: the length of sequence %d is negative or beyond its block table",
+                    word[2]);
+    }
   }
   return MPC_OK;
 }

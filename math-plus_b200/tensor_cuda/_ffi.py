@@ -21,6 +21,7 @@ STATUS_NAMES = {0: "OK", 1: "INVALID", 2: "UNSUPPORTED", 3: "OOM", 4: "CUDA", 5:
                 7: "NO_DEVICE", 8: "COMM", 9: "COMPILE"}
 # mpc_dtype
 F32, F16, BF16, I32, BOOL = range(5)
+E4M3 = 5  # MPC_E4M3: paged caches only
 FUSED_F32 = 1  # MPC_FUSED_F32
 DTYPE_CODES = {"f32": F32, "f16": F16, "bf16": BF16, "i32": I32, "bool": BOOL}
 DTYPE_BYTES = {F32: 4, F16: 2, BF16: 2, I32: 4, BOOL: 1}
@@ -59,6 +60,31 @@ class GemmDesc(C.Structure):
                 ("dtype_out", C.c_int32), ("b_layout", C.c_int32), ("epilogue", C.c_int32), ("alpha", C.c_float),
                 ("batch_rank", C.c_int32), ("batch_shape", C.c_int64 * 4), ("a_batch_stride", C.c_int64 * 4),
                 ("b_batch_stride", C.c_int64 * 4)]
+
+
+class KvDesc(C.Structure):
+    """mpc_kv_desc: the shape and storage of a paged key/value cache."""
+    _fields_ = [("n_pages", C.c_int64), ("page_size", C.c_int64), ("hk", C.c_int64), ("d", C.c_int64),
+                ("dv", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class KvTokens(C.Structure):
+    """mpc_kv_tokens: the dense rows of an append or a read."""
+    _fields_ = [("n", C.c_int64), ("n_seq", C.c_int64), ("max_pages", C.c_int64), ("k_stride", C.c_int64 * 2),
+                ("v_stride", C.c_int64 * 2), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class SdpaPagedDesc(C.Structure):
+    """mpc_sdpa_paged_desc."""
+    _fields_ = [("b", C.c_int64), ("h", C.c_int64), ("max_pages", C.c_int64), ("q_stride", C.c_int64 * 2),
+                ("o_stride", C.c_int64 * 2), ("dtype", C.c_int32), ("scale", C.c_float)]
+
+
+class SampleDesc(C.Structure):
+    """mpc_sample_desc."""
+    _fields_ = [("rows", C.c_int64), ("vocab", C.c_int64), ("row_stride", C.c_int64), ("dtype", C.c_int32),
+                ("top_k", C.c_int32), ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("reserved", C.c_int32)]
 
 
 class SdpaDesc(C.Structure):
@@ -132,6 +158,12 @@ SIGNATURES = {
     "mpc_gemm_f32_noalloc_status": [_vp],
     "mpc_gemm_f32_noalloc_selftest": [_u64, _vp],
     "mpc_sdpa": [_dev, C.POINTER(SdpaDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mpc_kv_append": [_dev, C.POINTER(KvDesc), _vp, _vp, _vp, _vp, C.POINTER(KvTokens), _vp, _vp, _vp, _vp, _vp, _vp],
+    "mpc_kv_read": [_dev, C.POINTER(KvDesc), _vp, _vp, _vp, _vp, C.POINTER(KvTokens), _vp, _vp, _vp, _vp, _vp, _vp],
+    "mpc_sdpa_paged_workspace": [_dev, C.POINTER(KvDesc), C.POINTER(SdpaPagedDesc), C.POINTER(_sz)],
+    "mpc_sdpa_paged": [_dev, C.POINTER(KvDesc), _vp, _vp, _vp, _vp, C.POINTER(SdpaPagedDesc), _vp, _vp, _vp, _vp, _vp,
+                       _vp, _sz, _vp],
+    "mpc_sample": [_dev, C.POINTER(SampleDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "mpc_softmax": [_dev, _vp, _i32, _vp, _i64, _i64, _i64, _vp],
     "mpc_gelu": [_dev, _vp, _i32, _vp, _i32, _i64, _vp],
     "mpc_add": [_dev, _vp, _vp, _vp, _i32, _i64, _i64, _vp],

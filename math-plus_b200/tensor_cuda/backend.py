@@ -750,6 +750,205 @@ class CudaBackend:
                C.c_void_p(base + 2 * E * eb), None, C.c_void_p(out._buf.ptr), None, C.byref(lay), None)
         return out
 
+    # ---- the paged key/value cache, single-token attention over it, sampling ----------------------
+    # (kv_cache.py; no counterpart in the reference)
+    def _mine(self, where: str, *ts) -> None:
+        """Live tensors of this device."""
+        self._check_live(*ts)
+        for t in ts:
+            if t is not None and t.backend.device is not self.device:
+                raise ValueError(f"tensor-cuda: {where}: tensor of another device (no implicit transfers)")
+
+    def _kv_tokens(self, where: str, cache, table: CudaTensor, pos: CudaTensor, seq: CudaTensor | None, n: int):
+        self._mine(where, table, pos, seq)
+        if cache.backend.device is not self.device:
+            raise ValueError(f"tensor-cuda: {where}: cache of another device (no implicit transfers)")
+        if cache.disposed:
+            raise RuntimeError(f"tensor-cuda: {where}: cache used after dispose")
+        for t, rank, name in ((table, 2, "table"), (pos, 1, "pos"), (seq, 1, "seq")):
+            if t is not None and (t.dtype != "i32" or len(t.shape) != rank):
+                raise TypeError(f"tensor-cuda: {where}: {name} is i32 of rank {rank}, got {t.dtype} "
+                                f"[{','.join(map(str, t.shape))}]")
+        if pos.shape[0] != n or (seq is not None and seq.shape[0] != n):
+            raise ValueError(f"tensor-cuda: {where}: {n} tokens, {pos.shape[0]} positions"
+                             + (f", {seq.shape[0]} sequence indices" if seq is not None else ""))
+        if seq is None and n > table.shape[0]:
+            raise ValueError(f"tensor-cuda: {where}: {n} tokens for {table.shape[0]} sequences need seq")
+        tok = F.KvTokens()
+        tok.n, tok.n_seq, tok.max_pages = n, table.shape[0], table.shape[1]
+        return tok
+
+    def kv_append(self, cache, k: CudaTensor, v: CudaTensor, table: CudaTensor, pos: CudaTensor,
+                  seq: CudaTensor | None = None) -> None:
+        """Writes token t's rows k[t] [Hk, D] and v[t] [Hk, Dv] at position pos[t] of sequence seq[t]
+        (default: sequence t) of a ``PagedKVCache``; pos < 0 is padding and writes nothing. k and v have the
+        cache's dtype, or any float dtype for an 8-bit cache. Two tokens of one call must not name the same
+        place. A place outside the cache is left out and raised by the next synchronisation."""
+        self._mine("kv_append", k, v)
+        if len(k.shape) != 3 or len(v.shape) != 3 or k.shape[1:] != (cache.n_kv_head, cache.head_dim) or \
+                v.shape != (k.shape[0], cache.n_kv_head, cache.head_dim_v):
+            raise ValueError(f"tensor-cuda: kv_append: k [{','.join(map(str, k.shape))}] v [{','.join(map(str, v.shape))}]"
+                             f" for {cache.n_kv_head} heads of {cache.head_dim} and {cache.head_dim_v}")
+        if k.dtype != v.dtype:
+            raise TypeError(f"tensor-cuda: kv_append: dtype mismatch {k.dtype} vs {v.dtype} (no implicit promotion)")
+        tok = self._kv_tokens("kv_append", cache, table, pos, seq, k.shape[0])
+        tok.k_stride[:] = [cache.n_kv_head * cache.head_dim, cache.head_dim]
+        tok.v_stride[:] = [cache.n_kv_head * cache.head_dim_v, cache.head_dim_v]
+        self._append(cache, tok, k.dtype, k.ptr, v.ptr, table, pos, seq)
+
+    def kv_append_packed(self, cache, qkv: CudaTensor, table: CudaTensor, pos: CudaTensor,
+                         seq: CudaTensor | None = None) -> None:
+        """``kv_append`` of K and V read in place from a packed projection qkv [T, (H + 2 Hk) D]: H query heads,
+        then the cache's K heads, then its V heads (``sdpa_packed``'s layout, with H = Hk)."""
+        self._mine("kv_append_packed", qkv)
+        n_q = self._packed_heads("kv_append_packed", cache, qkv)
+        tok = self._kv_tokens("kv_append_packed", cache, table, pos, seq, qkv.shape[0])
+        width, d = qkv.shape[1], cache.head_dim
+        tok.k_stride[:] = [width, d]
+        tok.v_stride[:] = [width, d]
+        eb = F.DTYPE_BYTES[F.DTYPE_CODES[qkv.dtype]]
+        k = qkv.ptr + n_q * d * eb
+        self._append(cache, tok, qkv.dtype, k, k + cache.n_kv_head * d * eb, table, pos, seq)
+
+    @staticmethod
+    def _packed_heads(where: str, cache, qkv: CudaTensor) -> int:
+        d, hk = cache.head_dim, cache.n_kv_head
+        n_q = qkv.shape[1] // d - 2 * hk if len(qkv.shape) == 2 else 0
+        if cache.head_dim_v != d or n_q <= 0 or qkv.shape[1] % d or n_q % hk:
+            raise ValueError(f"tensor-cuda: {where}: qkv [{','.join(map(str, qkv.shape))}] for {hk} K/V heads of {d} and "
+                             f"{cache.head_dim_v}")
+        return n_q
+
+    def _append(self, cache, tok, dtype: str, k: int, v: int, table, pos, seq) -> None:
+        if dtype not in FLOAT or (cache.dtype != "e4m3" and dtype != cache.dtype):
+            raise TypeError(f"tensor-cuda: kv_append: {dtype} rows into a {cache.dtype} cache (no implicit promotion)")
+        tok.dtype = F.DTYPE_CODES[dtype]
+        F.call("mpc_kv_append", self.device.handle, *cache.args, C.byref(tok), C.c_void_p(k), C.c_void_p(v),
+               C.c_void_p(table.ptr), C.c_void_p(seq.ptr if seq is not None else None), C.c_void_p(pos.ptr), None)
+
+    @staticmethod
+    def _check_out(where: str, out: CudaTensor, shape, dtype: str) -> CudaTensor:
+        if out.shape != tuple(shape) or out.dtype != dtype:
+            raise ValueError(f"tensor-cuda: {where}: out is {out.dtype} [{','.join(map(str, out.shape))}], the result "
+                             f"{dtype} [{','.join(map(str, shape))}]")
+        return out
+
+    def kv_read(self, cache, table: CudaTensor, pos: CudaTensor, seq: CudaTensor | None = None,
+                dtype: str | None = None, out=None):
+        """The rows at (seq[t], pos[t]) as dense (k [T, Hk, D], v [T, Hk, Dv]) of ``dtype`` (default: the cache's;
+        bf16 for an 8-bit cache), rounded once; zeros where pos < 0. ``out``: the (k, v) to write into."""
+        n = pos.shape[0] if pos.shape else 0
+        tok = self._kv_tokens("kv_read", cache, table, pos, seq, n)
+        dtype = dtype or ("bf16" if cache.dtype == "e4m3" else cache.dtype)
+        if dtype not in FLOAT:
+            raise TypeError(f"tensor-cuda: kv_read: float dtypes only, got {dtype}")
+        shapes = [(n, cache.n_kv_head, d) for d in (cache.head_dim, cache.head_dim_v)]
+        if out is None:
+            k, v = (self._alloc(s, dtype) for s in shapes)
+        else:
+            self._mine("kv_read", *out)
+            k, v = (self._check_out("kv_read", o, s, dtype) for o, s in zip(out, shapes))
+        tok.k_stride[:] = [shapes[0][1] * shapes[0][2], shapes[0][2]]
+        tok.v_stride[:] = [shapes[1][1] * shapes[1][2], shapes[1][2]]
+        tok.dtype = F.DTYPE_CODES[dtype]
+        F.call("mpc_kv_read", self.device.handle, *cache.args, C.byref(tok), C.c_void_p(k.ptr), C.c_void_p(v.ptr),
+               C.c_void_p(table.ptr), C.c_void_p(seq.ptr if seq is not None else None), C.c_void_p(pos.ptr), None)
+        return k, v
+
+    def sdpa_paged(self, q: CudaTensor, cache, table: CudaTensor, lengths: CudaTensor, scale: float, lse: bool = False,
+                   out=None):
+        """Attention of one new token per sequence, q [B, H, D], over the first lengths[b] rows of each sequence
+        of a ``PagedKVCache`` -> [B, H, Dv] (the ``sdpa`` of a decoding step; the new token's own row is one
+        of them, once appended). H is a multiple of the cache's heads (grouped-query attention). A length of 0
+        gives zeros. ``lse=True`` also returns the f32 [B, H] log-sum-exp. ``out``: what to write into (a pair
+        with ``lse``). Lengths or pages outside the cache are raised by the next synchronisation."""
+        self._mine("sdpa_paged", q)
+        if len(q.shape) != 3 or q.shape[2] != cache.head_dim:
+            raise ValueError(f"tensor-cuda: sdpa_paged: q [{','.join(map(str, q.shape))}] over head dim {cache.head_dim}")
+        B, H, D = q.shape
+        return self._sdpa_paged(q.ptr, q.dtype, (H * D, D), B, H, cache, table, lengths, scale, lse, out)
+
+    def sdpa_paged_packed(self, qkv: CudaTensor, cache, table: CudaTensor, lengths: CudaTensor, scale: float) -> CudaTensor:
+        """``sdpa_paged`` of the query heads of a packed projection qkv [B, (H + 2 Hk) D], read in place ->
+        [B, H D] with the heads merged (the decoding step of ``sdpa_packed``)."""
+        self._mine("sdpa_paged_packed", qkv)
+        H = self._packed_heads("sdpa_paged_packed", cache, qkv)
+        B, width = qkv.shape
+        o = self._sdpa_paged(qkv.ptr, qkv.dtype, (width, cache.head_dim), B, H, cache, table, lengths, scale, False, None)
+        merged = self.reshape(o, (B, H * cache.head_dim))
+        self.dispose(o)
+        return merged
+
+    def _sdpa_paged(self, q: int, dtype: str, q_stride, B: int, H: int, cache, table, lengths, scale, lse, out):
+        tok = self._kv_tokens("sdpa_paged", cache, table, lengths, None, B)
+        if table.shape[0] != B:
+            raise ValueError(f"tensor-cuda: sdpa_paged: {B} queries for {table.shape[0]} sequences")
+        if dtype not in FLOAT or (cache.dtype != "e4m3" and dtype != cache.dtype):
+            raise TypeError(f"tensor-cuda: sdpa_paged: {dtype} queries over a {cache.dtype} cache (no implicit promotion)")
+        if H % cache.n_kv_head:
+            raise ValueError(f"tensor-cuda: sdpa_paged: {H} heads over {cache.n_kv_head} K/V heads")
+        shape = (B, H, cache.head_dim_v)
+        if out is None:
+            o, z = self._alloc(shape, dtype), self._alloc((B, H), "f32") if lse else None
+        else:
+            o, z = out if lse else (out, None)
+            self._mine("sdpa_paged", o, z)
+            self._check_out("sdpa_paged", o, shape, dtype)
+            if z is not None:
+                self._check_out("sdpa_paged", z, (B, H), "f32")
+        desc = F.SdpaPagedDesc()
+        desc.b, desc.h, desc.max_pages = B, H, tok.max_pages
+        desc.q_stride[:] = q_stride
+        desc.o_stride[:] = (H * cache.head_dim_v, cache.head_dim_v)
+        desc.dtype, desc.scale = F.DTYPE_CODES[dtype], scale
+        F.call("mpc_sdpa_paged", self.device.handle, *cache.args, C.byref(desc), C.c_void_p(q), C.c_void_p(table.ptr),
+               C.c_void_p(lengths.ptr), C.c_void_p(o.ptr), C.c_void_p(z.ptr if z is not None else None), None, 0, None)
+        return (o, z) if lse else o
+
+    def sample(self, logits: CudaTensor, u: CudaTensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+               details: bool = False, out=None):
+        """One token per row of logits [B, V] from the uniform numbers u f32 [B]: i32 [B]. ``temperature``,
+        ``top_k``, ``top_p`` and ``min_p`` are numbers or per-row arrays (f32; top_k i32). Ranked by logit (ties:
+        lowest index first), the first top_k are kept, of those the ranks before which less than top_p of
+        their weight lies, of those the ones at least min_p times the best; the token is the lowest index
+        whose running sum of kept weights exceeds u times their total. temperature <= 0 takes the best token;
+        top_k <= 0, top_p >= 1, min_p <= 0 are off. A row with nothing above -inf gives -1. ``details=True``
+        also returns the token's probability in the kept set (f32 [B]) and the set's size (i32 [B])."""
+        self._mine("sample", logits)
+        if len(logits.shape) != 2 or not logits.shape[1]:
+            raise ValueError(f"tensor-cuda: sample: logits [{','.join(map(str, logits.shape))}], expected [B, V]")
+        if logits.dtype not in FLOAT:
+            raise TypeError(f"tensor-cuda: sample: float logits only, got {logits.dtype}")
+        B, V = logits.shape
+        desc = F.SampleDesc()
+        desc.rows, desc.vocab, desc.row_stride, desc.dtype = B, V, V, F.DTYPE_CODES[logits.dtype]
+        per_row = []
+        for name, x, dt in (("u", u, "f32"), ("temperature", temperature, "f32"), ("top_k", top_k, "i32"),
+                            ("top_p", top_p, "f32"), ("min_p", min_p, "f32")):
+            if isinstance(x, CudaTensor):
+                self._mine("sample", x)
+                if x.shape != (B,) or x.dtype != dt:
+                    raise TypeError(f"tensor-cuda: sample: {name} is {dt} [{B}], got {x.dtype} "
+                                    f"[{','.join(map(str, x.shape))}]")
+                per_row.append(C.c_void_p(x.ptr))
+            elif name == "u":
+                raise TypeError("tensor-cuda: sample: u is an f32 array, one uniform number per row")
+            else:
+                if name == "top_k":
+                    x = min(int(x), 0x7FFFFFFF) if x > 0 else 0
+                setattr(desc, name, x)
+                per_row.append(None)
+        if out is None:
+            outs = [self._alloc((B,), "i32")] + ([self._alloc((B,), "f32"), self._alloc((B,), "i32")] if details else [])
+        else:
+            outs = list(out) if details else [out]
+            self._mine("sample", *outs)
+            for o, dt in zip(outs, ("i32", "f32", "i32")):
+                self._check_out("sample", o, (B,), dt)
+        F.call("mpc_sample", self.device.handle, C.byref(desc), C.c_void_p(logits.ptr), *per_row,
+               *(C.c_void_p(o.ptr) for o in outs), *([None] * (3 - len(outs))), None)
+        return tuple(outs) if details else outs[0]
+
     def layerNorm(self, x: CudaTensor, weight: CudaTensor | None, bias: CudaTensor | None, eps: float = 1e-5):
         self._check_live(x, weight, bias)
         d = x.shape[-1]

@@ -1,0 +1,139 @@
+"""sample on the B200 against the definition in f64 on the host: tokens and kept sets equal, probabilities
+within f32 rounding."""
+import numpy as np
+import pytest
+
+from _paged import to_storage
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be():
+    from tensor_cuda.backend import CudaBackend
+    from tensor_cuda.runtime import Device
+    return CudaBackend(Device.shared(0))
+
+
+def up(be, arr, dtype):
+    from tensor_cuda.backend import host
+    return be.from_host_sync(host(dtype, np.shape(arr), np.asarray(arr)))
+
+
+def define(x, u, t, k, p, m):
+    """One row by the definition: (token, probability, size of the kept set)."""
+    x = np.where(np.isnan(x), -np.inf, x)
+    order = np.argsort(-x, kind="stable")
+    order = order[x[order] > -np.inf]
+    if not len(order):
+        return -1, 0.0, 0
+    if not t > 0:
+        return int(order[0]), 1.0, 1
+    if k > 0:
+        order = order[:k]
+    top = x[order[0]]
+    with np.errstate(invalid="ignore"):
+        d = (x[order] - top) / np.float64(t)
+    w = np.exp(np.where(x[order] == top, 0.0, np.where(np.isnan(d), -np.inf, d)))
+    keep = len(w)
+    if p < 1:
+        keep = max(1, int(np.sum(np.cumsum(w) - w < np.float64(p) * w.sum())))
+    keep = max(1, min(keep, int(np.sum(w >= np.float64(m)))))
+    order, w = order[:keep], w[:keep]
+    by = np.argsort(order)
+    c = np.cumsum(w[by])
+    u = min(max(float(u), 0.0), 1.0) if u == u else 0.0
+    j = int(np.searchsorted(c, u * c[-1], side="right"))
+    if j >= keep:
+        j = int(np.nonzero(w[by])[0][-1])
+    return int(order[by[j]]), w[by][j] / c[-1], keep
+
+
+def check(be, x, dtype, u, t=1.0, k=0, p=1.0, m=0.0):
+    raw, exact = to_storage(x, dtype)
+    B = x.shape[0]
+    row = lambda v, dt: np.broadcast_to(np.asarray(v, dt), (B,))  # noqa: E731
+    ts, ks, ps, ms = row(t, np.float32), row(k, np.int32), row(p, np.float32), row(m, np.float32)
+    dev = [v if np.ndim(v) == 0 else up(be, row(v, np.float32 if dt == "f32" else np.int32), dt)
+           for v, dt in ((t, "f32"), (k, "i32"), (p, "f32"), (m, "f32"))]
+    logits, ud = up(be, raw, dtype), up(be, np.asarray(u, np.float32), "f32")
+    tok, prob, kept = (be.read_sync(a).data for a in be.sample(logits, ud, *dev, details=True))
+    want = [define(exact[i], np.float32(u[i]), ts[i], int(ks[i]), ps[i], ms[i]) for i in range(B)]
+    wt, wp, wk = (np.array(v) for v in zip(*want))
+    assert np.array_equal(tok, wt), (tok, wt)
+    assert np.array_equal(kept, wk), (kept, wk)
+    # one rounding to f32; the sums are off by at most V 2^-47 of the total
+    assert np.all(np.abs(prob - wp) <= 2.0 ** -24 * wp * 1.01 + 1e-45 + x.shape[1] * 2.0 ** -47 * wp)
+    assert np.array_equal(be.read_sync(be.sample(logits, ud, *dev)).data, tok)
+
+
+def uniform(n, seed=0):
+    return np.random.default_rng(seed).random(n).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 1000, 1025, 4099, 50257])
+def test_settings_per_row(be, dtype, vocab):
+    r = np.random.default_rng(vocab)
+    B = 24
+    x = r.standard_normal((B, vocab)) * 3
+    x[:, 5::11] = -np.inf
+    check(be, x, dtype, uniform(B, 1), r.choice([0.0, 0.5, 1.0, 2.0], B), r.choice([0, 1, 2, 50, vocab, 10 ** 6], B),
+          r.choice([0.3, 0.9, 0.999, 1.0], B), r.choice([0.0, 0.01, 0.3, 1.0], B))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_large_vocabulary_without_filters_and_with_top_p(be, dtype):
+    x = np.random.default_rng(3).standard_normal((6, 200003)) * 2
+    check(be, x, dtype, uniform(6, 2))
+    check(be, x, dtype, uniform(6, 3), p=0.95)
+    check(be, x, dtype, uniform(6, 4), k=100000)
+
+
+def test_ties_go_to_the_lowest_index(be):
+    """Rows of equal logits, and of few distinct values: borders of top-k and top-p inside a tie."""
+    B = 12
+    x = np.zeros((B, 5000))
+    for k, p in ((0, 1.0), (7, 1.0), (0, 0.5), (4999, 0.25), (1, 0.01)):
+        check(be, x, "f32", uniform(B, k), k=k, p=p)
+    x = np.random.default_rng(1).integers(-3, 4, (B, 5000)).astype(np.float64)
+    for k, p, m in ((0, 1.0, 0.0), (300, 1.0, 0.0), (2000, 0.7, 0.0), (0, 0.6, 0.1), (0, 1.0, 1.0)):
+        check(be, x, "f16", uniform(B, k), k=k, p=p, m=m)
+    check(be, np.array([[-0.0, 0.0, -0.0, 0.0]] * 4), "f32", [0.1, 0.3, 0.6, 0.9], k=2)
+
+
+def test_rows_without_tokens_and_extreme_logits(be):
+    inf, nan = np.inf, np.nan
+    x = np.array([[-inf] * 6, [nan] * 6, [nan, -inf, 3, nan, -inf, nan], [inf, 1, inf, 2, -inf, 0],
+                  [3e38, -3e38, 0, 3e38, 1, -inf], [-3e38, -inf, -3.1e38, nan, -inf, -3e38], [0, -200, -1000, 5, -800, 5]])
+    for u in (0.0, 0.49, 0.51, 0.999):
+        us = [u] * len(x)
+        check(be, x, "f32", us)
+        check(be, x, "f32", us, t=0.0)
+        check(be, x, "f32", us, k=2, p=0.9)
+        check(be, x, "f32", us, t=1e-6)
+        check(be, x, "f32", us, t=1e6, p=0.4, m=0.5)
+        check(be, x, "bf16", us, t=np.inf)
+
+
+def test_ends_of_the_settings(be):
+    x = np.random.default_rng(5).standard_normal((4, 300)) * 2
+    u = [0.0, 1.0 - 2.0 ** -24, 1.0, 7.0]
+    check(be, x, "f32", u)
+    check(be, x, "f32", [-1.0, np.nan, 0.5, 0.2], p=0.8)
+    check(be, x, "f32", u, p=0.0)
+    check(be, x, "f32", u, p=-1.0, k=-5)
+    check(be, x, "f32", u, m=2.0)
+    check(be, x, "f32", u, t=np.nan)
+    check(be, x, "f32", u, t=-1.0)
+
+
+def test_draws_follow_the_weights(be):
+    """Evenly spaced u give each token its share of the rows, within one row."""
+    n = 2000
+    logits = np.log(np.array([0.5, 0.25, 0.125, 0.0625, 0.0625]))
+    x = np.broadcast_to(logits, (n, 5)).copy()
+    u = (np.arange(n) + 0.5) / n
+    tok = be.read_sync(be.sample(up(be, x.astype(np.float32), "f32"), up(be, u.astype(np.float32), "f32"))).data
+    share = np.bincount(tok, minlength=5)
+    assert np.all(np.abs(share - np.exp(logits) * n) <= 1.5)
