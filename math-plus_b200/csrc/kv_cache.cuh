@@ -28,6 +28,12 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(two));
   return r;
 }
+// Four of them, as two f16x2.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t &lo, uint32_t &hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
 __device__ __forceinline__ float2 f16x2_to_f32(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
@@ -43,7 +49,9 @@ __device__ __forceinline__ uint32_t f32_to_bf16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ void e4m3x4_to_f32(uint32_t v, float *x) {
-  const float2 a = f16x2_to_f32(e4m3x2_to_f16x2(v & 0xffffu)), b = f16x2_to_f32(e4m3x2_to_f16x2(v >> 16));
+  uint32_t lo, hi;
+  e4m3x4_to_f16x4(v, lo, hi);
+  const float2 a = f16x2_to_f32(lo), b = f16x2_to_f32(hi);
   x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 // Round to nearest even, saturating at 448; NaN gives NaN.

@@ -5,26 +5,35 @@
 // upper reference of s' (the running maximum). Every K/V row is read once and used for the query
 // heads that share it, so the cache's bytes bound the time and the work is split along the cache:
 //
-// Split. An item is (sequence, K/V head, tile of its query heads); its keys are cut into chunks of 64.
-// The chunks of all items, in order, are dealt to the CTAs in equal runs: CTA i of n takes chunks
-// [T i / n, T (i + 1) / n). Each CTA finds its run from the lengths on the device, so ragged batches and a
-// single long sequence balance alike and the launch depends on host-known sizes alone (it can be
-// captured into a graph). A run that covers an item wholly writes the output; otherwise the (at
-// most two) cut items of a CTA leave (m, l, O) in the workspace and a second kernel joins them in
-// CTA order, so the result does not depend on timing.
+// Split. An item is (sequence, K/V head, tile of its query heads); its keys are cut into tiles (16 or 32). The
+// tiles of all items, in order, with kItemCost more for every item (an item's start and end take about
+// as long as that many tiles), are dealt to the warps in equal runs: warp i of n takes units [T i / n,
+// T (i + 1) / n). The runs are found from the lengths on the device, so ragged batches and a single long
+// sequence balance alike and the launch depends on host-known sizes alone (it can be captured into a
+// graph). A warp that has an item wholly writes the output. Otherwise the (at most two) cut items of
+// a warp leave (m, l, O) in the workspace, one for the block where all its warps are inside one item, and a
+// second kernel joins them in order, so the result does not depend on timing.
 //
-// CUDA-core kernel (f32 rows, and any head dim <= 256 or alignment): 8 lanes per key, 4 keys a warp, each
-// group of 8 lanes with its own running maximum, sum and O; the 16 groups of a CTA meet once per item.
+// CUDA-core kernel (f32 rows, and any head dim <= 256 or alignment): 8 lanes per key, 4 keys at a time, each
+// group of 8 lanes with its own running maximum, sum and O, which meet once per item.
 #include <cfloat>
 
 #include "kv_cache.cuh"
 #include "mpc_internal.h"
+#include "sm100.cuh"
 
 namespace mpc {
 namespace paged {
 
-constexpr int kChunk = 64;     // keys of one unit of the split
-constexpr int kThreads = 128;  // 4 warps
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+#ifndef ITEM_COST
+#define ITEM_COST 3
+#define E4_TPI 2
+#define E4_MINB 2
+#define D64_TPI 2
+#define D64_MINB 3
+#endif
+constexpr int kItemCost = ITEM_COST;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -33,45 +42,60 @@ struct Params {
   const int32_t *table, *lengths;
   void *out;
   float *lse, *ws;
+  int4 *owners;  // per warp: (sequence, head tile, last warp, unused) of the item it starts and another ends; last -1: none
   int *err;
   long long qs[2], os[2], max_pages, cap;  // cap: max_pages * page_size
-  int B, H, hk, group, gt, qt;  // query heads per K/V head, per tile, tiles per K/V head
+  int B, H, hk, group, gt, qt, tile;  // query heads per K/V head, per query tile; tiles per K/V head; keys of a tile
   int d, dv, page_size, n_pages, dt, dt_pages;
+  uint32_t page_mul, page_shift;  // key / page_size = key * page_mul >> page_shift for keys below 2^31
   float scale_log2;
+  __device__ __forceinline__ unsigned page_of(unsigned key) const { return (unsigned)((uint64_t)key * page_mul >> page_shift); }
 };
 
-// The run of chunks of one CTA, found from the lengths.
-struct Run {
-  long long total, g0, g1;  // all chunks; this CTA's [g0, g1)
-  int n;                    // CTAs that have a run
-};
+// A warp's place in an item. All units of a call are fewer than 2^31 (plan_of).
 struct Item {
-  int b, head;        // head: K/V head * qt + query tile
-  long long chunk, chunks;
+  int b, head;       // head: K/V head * qt + query tile
+  int start, units;  // the item's first unit and its units: kItemCost, then one per tile
 };
 
-__device__ __forceinline__ long long length_of(const Params &p, int b) {
-  const long long len = p.lengths[b];
-  return len < 0 ? 0 : len > p.cap ? p.cap : len;
+__device__ __forceinline__ int length_of(const Params &p, int b) {
+  const int len = p.lengths[b];
+  return len < 0 ? 0 : len > p.cap ? (int)p.cap : len;
 }
-__device__ __forceinline__ long long chunks_of(const Params &p, int b) {
-  return (length_of(p, b) + kChunk - 1) / kChunk;
+__device__ __forceinline__ int units_of(const Params &p, int b) {
+  const int len = length_of(p, b);
+  return len ? (int)((unsigned)(len - 1) / (unsigned)p.tile) + 1 + kItemCost : 0;
 }
 
-// Block-wide inclusive scan of one value a thread (kThreads threads); *sum: the block's total.
-__device__ __forceinline__ long long scan(long long v, long long *sm, long long *sum) {
+// `total` units dealt to n warps: the first `more` have each + 1.
+struct Deal {
+  int total, n, each, more;
+  __device__ __forceinline__ void set(int units, int warps) {
+    total = units, n = min(units, warps);
+    each = n ? (unsigned)total / (unsigned)n : 0;
+    more = total - each * n;
+  }
+  __device__ __forceinline__ int start(int warp) const { return warp * each + min(warp, more); }
+  __device__ __forceinline__ int warp_of(int unit) const {
+    const int cut = more * (each + 1);
+    return unit < cut ? (unsigned)unit / (unsigned)(each + 1) : more + (unsigned)(unit - cut) / (unsigned)each;
+  }
+};
+
+// Block-wide inclusive scan of one value a thread; *sum: the block's total.
+__device__ __forceinline__ int scan(int v, int *sm, int *sum) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, m);
+    const int u = __shfl_up_sync(0xffffffffu, v, m);
     if (lane >= m) v += u;
   }
   __syncthreads();
   if (lane == 31) sm[w] = v;
   __syncthreads();
-  long long before = 0, all = 0;
+  int before = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) {
+  for (int i = 0; i < kWarps; ++i) {
     if (i < w) before += sm[i];
     all += sm[i];
   }
@@ -79,52 +103,53 @@ __device__ __forceinline__ long long scan(long long v, long long *sm, long long 
   return v + before;
 }
 
-__device__ __forceinline__ Run run_of(const Params &p, int cta, int ctas, long long *sm) {
-  long long total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    long long sum;
-    scan(b < p.B ? chunks_of(p, b) : 0, sm, &sum);
-    total += sum;
+// The deal and the item of the block's first unit, by a scan of the lengths, kThreads sequences at a time: once
+// where that is all of them. sm: kWarps + 2. Returns whether the block has a run.
+__device__ __forceinline__ bool find_run(const Params &p, int *sm, Deal &deal, Item &it) {
+  const int heads = p.hk * p.qt;
+  int own = threadIdx.x < p.B ? units_of(p, threadIdx.x) * heads : 0, sum;
+  int incl = scan(own, sm, &sum), total = sum;
+  for (int b0 = kThreads; b0 < p.B; b0 += kThreads) {
+    int more;
+    scan(b0 + (int)threadIdx.x < p.B ? units_of(p, b0 + threadIdx.x) * heads : 0, sm, &more);
+    total += more;
   }
-  Run r;
-  r.total = total * (p.hk * p.qt);
-  r.n = (int)(r.total < ctas ? r.total : ctas);
-  if (cta >= r.n) {
-    r.g0 = r.g1 = 0;
-  } else {
-    r.g0 = r.total * cta / r.n;
-    r.g1 = r.total * (cta + 1) / r.n;
-  }
-  return r;
-}
-
-// The item of chunk g (0 <= g < total) and g's place in it.
-__device__ __forceinline__ Item item_of(const Params &p, long long g, long long *sm, long long *found) {
-  const long long heads = p.hk * p.qt;
-  long long before = 0;
+  deal.set(total, gridDim.x * kWarps);
+  const int w0 = blockIdx.x * kWarps;
+  if (w0 >= deal.n) return false;
+  const int c0 = deal.start(w0);
+  int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const long long c = b < p.B ? chunks_of(p, b) : 0;
-    long long sum;
-    const long long incl = before + scan(c, sm, &sum);
-    if (g >= (incl - c) * heads && g < incl * heads) found[0] = b, found[1] = incl - c;
+    if (b0) {
+      own = b0 + (int)threadIdx.x < p.B ? units_of(p, b0 + threadIdx.x) * heads : 0;
+      incl = before + scan(own, sm, &sum);
+    }
+    if (c0 >= incl - own && c0 < incl) sm[kWarps] = b0 + threadIdx.x, sm[kWarps + 1] = incl - own;
     before += sum;
   }
   __syncthreads();
-  Item it;
-  it.b = (int)found[0];
-  const long long rem = g - found[1] * heads;
-  it.chunks = chunks_of(p, it.b);
-  it.head = (int)(rem / it.chunks);
-  it.chunk = rem - it.head * it.chunks;
-  return it;
+  it.b = sm[kWarps];
+  it.units = units_of(p, it.b);
+  const int rem = c0 - sm[kWarps + 1];
+  it.head = (unsigned)rem / (unsigned)it.units;
+  it.start = c0 - (rem - it.head * it.units);
+  return true;
+}
+
+__device__ __forceinline__ void advance(const Params &p, Item &it) {
+  it.start += it.units;
+  if (++it.head == p.hk * p.qt) {
+    it.head = 0;
+    do it.units = units_of(p, ++it.b);
+    while (it.units == 0);  // only called where a later unit exists
+  }
 }
 
 // (m, l, O) of one query over part of an item, in the workspace: m, the exponent O refers to, l, one
-// unused, then O.
-__device__ __forceinline__ float *slot(const Params &p, int cta, bool first, int g) {
-  return p.ws + ((long long)(2 * cta + (first ? 1 : 0)) * p.gt + g) * (p.dv + 4);
+// unused, then O, in whole 16 bytes. A warp's part at the item's start and one further on have a place each.
+__host__ __device__ __forceinline__ int slot_floats(int dv) { return (dv + 3) / 4 * 4 + 4; }
+__device__ __forceinline__ float *slot(const Params &p, int warp, bool first, int q) {
+  return p.ws + (long long)((2 * warp + (first ? 1 : 0)) * p.gt + q) * slot_floats(p.dv);
 }
 
 __device__ __forceinline__ float guard_exp2(float x, float ref) { return x == -INFINITY ? 0.0f : exp2f(x - ref); }
@@ -132,7 +157,7 @@ __device__ __forceinline__ float guard_exp2(float x, float ref) { return x == -I
 // Sequences without keys: zeros and -inf; lengths outside the table are recorded.
 __device__ __forceinline__ void empty_rows(const Params &p) {
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    const long long len = p.lengths[b];
+    const int len = p.lengths[b];
     if (threadIdx.x == 0 && (len < 0 || len > p.cap)) report_bad_page(p.err, kBadLength, b);
     if (len > 0 && p.cap > 0) continue;
     for (int i = threadIdx.x; i < p.H * p.dv; i += kThreads) {
@@ -144,29 +169,131 @@ __device__ __forceinline__ void empty_rows(const Params &p) {
   }
 }
 
+__device__ __forceinline__ void put(const Params &p, int b, int h, int e, float v, float sum, float top, float otop) {
+  store_f32(p.out, p.dt, b * p.os[0] + h * p.os[1] + e, sum != 0.0f ? v * exp2f(otop - top) / sum : 0.0f);
+  if (p.lse && e == 0) p.lse[(long long)b * p.H + h] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+}
+
+// Column e of query q over the results of SRC warps: (m, the exponent O refers to, l) in sml[src][q], O in so[src][q].
+template <int SRC, int GT, int PITCH>
+__device__ __forceinline__ void combine(const float (*so)[GT][PITCH], const float (*sml)[GT][3], int q, int e, float &v,
+                                        float &sum, float &top, float &otop) {
+  top = otop = -INFINITY, sum = v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < SRC; ++w) top = fmaxf(top, sml[w][q][0]), otop = fmaxf(otop, sml[w][q][1]);
+#pragma unroll
+  for (int w = 0; w < SRC; ++w) {
+    sum = fmaf(sml[w][q][2], guard_exp2(sml[w][q][0], top), sum);
+    v = fmaf(so[w][q][e], guard_exp2(sml[w][q][1], otop), v);
+  }
+}
+
+// Sends tiles [t0, t1) of an item on: to the output where that is all of it, else to the workspace. The
+// results of SRC warps are in shared memory; `threads` threads of which this is `id` do it for warp `gw`.
+template <int SRC, int GT, int PITCH>
+__device__ __forceinline__ void finish(const Params &p, const Item &it, int t0, int t1, int gw,
+                                       const float (*so)[GT][PITCH], const float (*sml)[GT][3], int id, int threads) {
+  const int kvh = it.head / p.qt, h0 = kvh * p.group + (it.head % p.qt) * GT;
+  const int nq = min(GT, (kvh + 1) * p.group - h0);
+  const bool whole = t0 == 0 && t1 == it.units - kItemCost;
+  const int w4 = (p.dv + 31) / 32 * 32;  // whole warps per query
+  for (int i = id; i < nq * w4; i += threads) {
+    const int q = i / w4, e = i - q * w4;
+    if (e >= p.dv) continue;
+    float top, otop, sum, v;
+    combine<SRC>(so, sml, q, e, v, sum, top, otop);
+    if (whole) {
+      put(p, it.b, h0 + q, e, v, sum, top, otop);
+    } else {
+      float *ws = slot(p, gw, t0 == 0, q);
+      ws[4 + e] = v;
+      if (e == 0) *reinterpret_cast<float4 *>(ws) = make_float4(top, otop, sum, 0.0f);
+    }
+  }
+}
+
+// Walks a warp's run: body(sequence, head tile, t0, t1) leaves its part of each item in shared memory. The place
+// in the run is in shared memory too, while the body has the registers.
+template <int GT, int PITCH, typename Body>
+__device__ __forceinline__ void walk(const Params &p, float (*so)[GT][PITCH], float (*sml)[GT][3], Body body) {
+  struct Place {
+    Item it;
+    int u, u1;  // the unit the warp is at, the end of its run
+  };
+  __shared__ int sm[kWarps + 2];
+  __shared__ Place places[kWarps];
+  __shared__ Deal all;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gw = blockIdx.x * kWarps + warp;
+  volatile Place *const here = &places[warp];
+  bool meet = false;  // the block is inside one item: its warps meet at the end
+  bool go = false;
+  {
+    Deal deal;
+    Item it{};
+    int u0 = 0, u1 = 0;
+    if (find_run(p, sm, deal, it)) {
+      meet = deal.start(min(gw - warp + kWarps, deal.n)) <= it.start + it.units;
+      if (gw < deal.n) u0 = deal.start(gw), u1 = deal.start(gw + 1);
+      go = u0 < u1 || meet;
+      if (!meet && go)
+        while (it.start + it.units <= u0) advance(p, it);
+    }
+    if (lane == 0) {
+      places[warp].it = it, places[warp].u = u0, places[warp].u1 = u1;
+      p.owners[gw] = make_int4(0, 0, -1, 0);
+      if (warp == 0) all = deal;
+    }
+  }
+  __syncthreads();
+  grid_dependents_launch();  // every block is running by now: the join's blocks may take the places that become free
+  while (go) {
+    int u = here->u, end = min(here->u1, here->it.start + here->it.units), base = here->it.start + kItemCost;
+    if (meet || end > base) body(here->it.b, here->it.head, max(0, u - base), max(0, end - base));
+    __syncwarp();
+    Item it;
+    it.b = here->it.b, it.head = here->it.head, it.start = here->it.start, it.units = here->it.units;
+    const int u1 = here->u1;
+    u = here->u, end = min(u1, it.start + it.units), base = it.start + kItemCost;
+    int from = max(0, u - base), to = max(0, end - base);
+    if (meet) {
+      __syncthreads();
+      if (warp && lane < GT && u < u1)  // the block's part goes to its first warp's place
+        *reinterpret_cast<float4 *>(slot(p, gw, false, lane)) = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+      const int w0 = gw - warp;
+      from = max(0, all.start(w0) - base), to = max(0, all.start(min(w0 + kWarps, all.n)) - base);
+      if (to > from) finish<kWarps, GT, PITCH>(p, it, from, to, w0, so, sml, threadIdx.x, kThreads);
+    } else if (to > from) {
+      finish<1, GT, PITCH>(p, it, from, to, gw, so + warp, sml + warp, lane, 32);
+    }
+    if (lane == 0 && (!meet || warp == 0) && from == 0 && to > 0 && to < it.units - kItemCost)
+      p.owners[gw] = make_int4(it.b, it.head, all.warp_of(it.start + it.units - 1), 0);
+    go = !meet && end < u1;
+    __syncwarp();
+    if (go) {
+      advance(p, it);
+      if (lane == 0) places[warp].it = it, places[warp].u = end;
+      __syncwarp();
+    }
+  }
+  empty_rows(p);
+}
+
 // ---- CUDA-core kernel ---------------------------------------------------------------------------
 template <int NI, int GT, bool VEC>
 __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
   constexpr int W = NI * 64;  // padded head dim: lane j of 8 holds values i * 64 + j * 8 ..+7
-  __shared__ float sq[GT][W];
-  __shared__ float so[kThreads / 32][GT][W];
-  __shared__ float sml[kThreads / 32][GT][2];
-  __shared__ long long sm[kThreads / 32], found[2];
-  empty_rows(p);
-  const Run run = run_of(p, blockIdx.x, gridDim.x, sm);
-  if (run.g0 >= run.g1) return;
-  Item it = item_of(p, run.g0, sm, found);
+  __shared__ float sq[kWarps][GT][W];
+  __shared__ float so[kWarps][GT][W];
+  __shared__ float sml[kWarps][GT][3];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j8 = (lane & 7) * 8;
-  for (long long g = run.g0; g < run.g1;) {
-    const long long c1 = min(it.chunks, it.chunk + (run.g1 - g));
-    const int kvh = it.head / p.qt, h0 = kvh * p.group + (it.head % p.qt) * GT;
+  walk<GT, W>(p, so, sml, [&](int b, int head, int t0, int t1) {
+    const int kvh = head / p.qt, h0 = kvh * p.group + (head % p.qt) * GT;
     const int nq = min(GT, (kvh + 1) * p.group - h0);
-    __syncthreads();  // the last item's shared arrays are free
-    for (int i = threadIdx.x; i < GT * W; i += kThreads) {
+    for (int i = lane; i < GT * W; i += 32) {
       const int q = i / W, e = i % W;
-      sq[q][e] = q < nq && e < p.d ? load_f32(p.q, p.dt, it.b * p.qs[0] + (h0 + q) * p.qs[1] + e) : 0.0f;
+      sq[warp][q][e] = q < nq && e < p.d ? load_f32(p.q, p.dt, b * p.qs[0] + (h0 + q) * p.qs[1] + e) : 0.0f;
     }
-    __syncthreads();
+    __syncwarp();
     float m[GT], l[GT], o[GT][NI * 8];
 #pragma unroll
     for (int q = 0; q < GT; ++q) {
@@ -174,15 +301,15 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < NI * 8; ++e) o[q][e] = 0.0f;
     }
-    const long long end = min(length_of(p, it.b), c1 * kChunk);
-    for (long long k0 = it.chunk * kChunk; k0 < end; k0 += kThreads / 8) {
-      const long long key = k0 + (threadIdx.x >> 3);
+    const unsigned end = (unsigned)min((long long)length_of(p, b), (long long)t1 * p.tile);  // lengths are below 2^31
+    for (unsigned k0 = (unsigned)t0 * (unsigned)p.tile; k0 < end; k0 += 4) {
+      const unsigned key = k0 + (lane >> 3);
       long long row = -1;
       if (key < end) {
-        const long long col = key / p.page_size;
-        const int pg = p.table[it.b * p.max_pages + col];
-        if (pg >= 0 && pg < p.n_pages) row = ((long long)pg * p.hk + kvh) * p.page_size + (key - col * p.page_size);
-        else if ((lane & 7) == 0) report_bad_page(p.err, kBadAttend, it.b);
+        const unsigned col = p.page_of(key);
+        const int pg = p.table[(long long)b * p.max_pages + col];
+        if (pg >= 0 && pg < p.n_pages) row = ((long long)pg * p.hk + kvh) * p.page_size + (key - col * (unsigned)p.page_size);
+        else if ((lane & 7) == 0) report_bad_page(p.err, kBadAttend, b);
       }
       float s[GT], x[8];
 #pragma unroll
@@ -195,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 #pragma unroll
           for (int q = 0; q < GT; ++q)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[q] = fmaf(sq[q][at + e], x[e], s[q]);
+            for (int e = 0; e < 8; ++e) s[q] = fmaf(sq[warp][q][at + e], x[e], s[q]);
         }
       }
 #pragma unroll
@@ -230,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
         }
       }
     }
-    // The 4 groups of a warp meet by shuffles, the warps in shared memory.
+    // The 4 groups of the warp meet by shuffles.
 #pragma unroll
     for (int q = 0; q < GT; ++q) {
       float top = m[q];
@@ -247,40 +374,9 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
         for (int k = 8; k < 32; k <<= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
         if (lane < 8) so[warp][q][(e >> 3) * 64 + j8 + (e & 7)] = v;
       }
-      if (lane == 0) sml[warp][q][0] = top, sml[warp][q][1] = l[q];
+      if (lane == 0) sml[warp][q][0] = sml[warp][q][1] = top, sml[warp][q][2] = l[q];
     }
-    __syncthreads();
-    const bool whole = it.chunk == 0 && c1 == it.chunks;
-    for (int i = threadIdx.x; i < nq * W; i += kThreads) {
-      const int q = i / W, e = i % W;
-      float top = -INFINITY, sum = 0.0f, v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, sml[w][q][0]);
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) {
-        const float keep = guard_exp2(sml[w][q][0], top);
-        sum = fmaf(sml[w][q][1], keep, sum);
-        v = fmaf(so[w][q][e], keep, v);
-      }
-      if (whole) {
-        if (e < p.dv)
-          store_f32(p.out, p.dt, it.b * p.os[0] + (h0 + q) * p.os[1] + e, sum != 0.0f ? v / sum : 0.0f);
-        if (p.lse && e == 0) p.lse[(long long)it.b * p.H + h0 + q] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
-      } else {
-        float *ws = slot(p, blockIdx.x, it.chunk == 0, q);
-        if (e < p.dv) ws[4 + e] = v;
-        if (e == 0) ws[0] = ws[1] = top, ws[2] = sum;
-      }
-    }
-    g += c1 - it.chunk;
-    it.chunk = 0;
-    if (++it.head == p.hk * p.qt) {
-      it.head = 0;
-      if (g < run.g1)
-        do it.chunks = chunks_of(p, ++it.b);
-        while (it.chunks == 0);
-    }
-  }
+  });
 }
 
 // ---- tensor-core kernel ---------------------------------------------------------------------------
@@ -298,7 +394,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 //      that the products want are byte permutes of two such registers.
 // Weights: S^T's layout transposed (movmatrix) is P^T's. A weight goes in as the sum of two numbers of the
 // type (its rounding and the rest), which leaves 2^-16 (bf16) or less of it; one number alone would add
-// as much error as the output's own rounding.
+// as much error as the output's own rounding. Over 8-bit rows the weights are f16, and where the output is
+// bf16 their rounding of 2^-12 is an eighth of the output's, so one number does.
 // The reference m of the exponentials is only raised when a score passes it by more than 2^kSlack: a warp
 // vote per tile in the common case, the row maximum by shuffles and a rescaling of O else. It is set 2^kHead
 // below the maximum so that small weights stay clear of f16's subnormals.
@@ -307,6 +404,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 // score. V's joins the weight: w = 2^(s' + e_v - M) with a reference M of its own, so that rows far below
 // the largest scale keep their precision.
 constexpr float kHead = 6.0f, kSlack = 14.0f;
+constexpr float kNoRef = -3e38f;  // the reference before any score; 2^(-inf - kNoRef) is 0
 constexpr uint32_t kNoRow = 0xffffffffu;
 enum { kF16, kBF16, kE4M3 };
 
@@ -333,98 +431,130 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return r;
 }
 
-// 8 values of a row as loaded: 4 registers of 16-bit pairs, or 2 of 8-bit codes.
+// 2^x, 0 for -inf.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 8 values of a row as loaded: 4 registers of 16-bit pairs, or 2 of 8-bit codes. Zero from the start, they stay so
+// where the row is shorter (`in` never changes).
 template <int KIND>
 struct Chunk {
   static constexpr int N = KIND == kE4M3 ? 2 : 4;
   uint32_t r[N];
-  __device__ __forceinline__ void load(const void *base, uint32_t row, int d, int at) {
-    const bool there = row != kNoRow && at < d;
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = 0;
+  }
+  __device__ __forceinline__ void load(const uint8_t *at, bool in) {
     if constexpr (KIND == kE4M3) {
-      uint2 v = make_uint2(0, 0);
-      if (there) v = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(base) + (size_t)row * d + at));
-      r[0] = v.x, r[1] = v.y;
+      if (in) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at));
+        r[0] = v.x, r[1] = v.y;
+      }
     } else {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (there) v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + (size_t)row * d + at));
-      r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+      if (in) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at));
+        r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+      }
     }
   }
-  // Values 2i and 2i + 1 as a pair.
-  __device__ __forceinline__ uint32_t pair(int i) const {
-    if constexpr (KIND == kE4M3) return e4m3x2_to_f16x2((i & 1) ? r[i >> 1] >> 16 : r[i >> 1] & 0xffffu);
-    else return r[i];
+  // Values 0, 1 | 2, 3 | 4, 5 | 6, 7 as pairs.
+  __device__ __forceinline__ void pairs(uint32_t (&x)[4]) const {
+    if constexpr (KIND == kE4M3) {
+      e4m3x4_to_f16x4(r[0], x[0], x[1]);
+      e4m3x4_to_f16x4(r[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = r[i];
+    }
   }
 };
 // Value 2i (a0) and 2i + 1 (a1) of two neighbouring keys, as pairs (key, next key).
 template <int KIND>
 __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND> &y, int i, uint32_t &a0, uint32_t &a1) {
   if constexpr (KIND == kE4M3) {
-    const uint32_t t = prmt(x.r[i >> 1], y.r[i >> 1], (i & 1) ? 0x7362u : 0x5140u);
-    a0 = e4m3x2_to_f16x2(t & 0xffffu);
-    a1 = e4m3x2_to_f16x2(t >> 16);
+    e4m3x4_to_f16x4(prmt(x.r[i >> 1], y.r[i >> 1], (i & 1) ? 0x7362u : 0x5140u), a0, a1);
   } else {
     a0 = prmt(x.r[i], y.r[i], 0x5410u);
     a1 = prmt(x.r[i], y.r[i], 0x7632u);
   }
 }
 
-// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value.
-template <int KIND, int DP, int NT, int QS>
-__global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_kernel(const Params p) {
+// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value; LO: weights as two
+// numbers. TPI tiles of 16
+// keys at a time: 32 keys where their rows fit the registers that 16 longer ones take.
+template <int KIND, int DP>
+constexpr int tiles_at_once() { return DP == 64 ? D64_TPI : (DP == 128 && KIND == kE4M3) ? E4_TPI : 1; }
+
+template <int KIND, int DP, int NT, int QS, bool LO>
+__global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : DP == 64 ? D64_MINB : KIND == kE4M3 ? E4_MINB : 3) mma_kernel(const Params p) {
   constexpr bool BF = KIND == kBF16, Q8 = KIND == kE4M3;
-  constexpr int KC = DP / 32, VC = DP / 64, GT = 8 * NT, PITCH = DP + 8, WARPS = kThreads / 32;
-  __shared__ float so[WARPS][GT][PITCH];
-  __shared__ float sml[WARPS][GT][3];
-  __shared__ long long sm[WARPS], found[2];
-  empty_rows(p);
-  const Run run = run_of(p, blockIdx.x, gridDim.x, sm);
-  if (run.g0 >= run.g1) return;
-  Item it = item_of(p, run.g0, sm, found);
+  constexpr int KC = DP / 32, VC = DP / 64, GT = 8 * NT, PITCH = DP + 8, TPI = tiles_at_once<KIND, DP>(), KEYS = 16 * TPI;
+  __shared__ alignas(16) float so[kWarps][GT][PITCH];  // written as pairs
+  __shared__ float sml[kWarps][GT][3];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
 
-  for (long long g = run.g0; g < run.g1;) {
-    const long long c1 = min(it.chunks, it.chunk + (run.g1 - g));
-    const int kvh = it.head / p.qt, h0 = kvh * p.group + (it.head % p.qt) * GT;
+  walk<GT, PITCH>(p, so, sml, [&](int b, int head, int t0, int t1) {
+    const int kvh = head / p.qt, h0 = kvh * p.group + (head % p.qt) * GT;
     const int nq = min(GT, (kvh + 1) * p.group - h0);
-    const unsigned end = (unsigned)min(length_of(p, it.b), c1 * kChunk);  // lengths are below 2^31
-    const int32_t *table = p.table + it.b * p.max_pages;
+    const unsigned end = (unsigned)min((long long)length_of(p, b), (long long)t1 * p.tile);  // lengths are below 2^31
+    const int32_t *table = p.table + (long long)b * p.max_pages;
 
-    // The row of this lane's key (lane % 16) in the tile of keys from k0 on.
+    // The row of this lane's key (lane % KEYS) in the tile of keys from k0 on.
     auto row_at = [&](unsigned k0) -> uint32_t {
-      const unsigned key = k0 + (lane & 15);
+      const unsigned key = k0 + (lane & (KEYS - 1));
       if (key >= end) return kNoRow;
-      const unsigned col = key / (unsigned)p.page_size;
+      const unsigned col = p.page_of(key);
       const int pg = __ldg(table + col);
       if (pg < 0 || pg >= p.n_pages) {
-        report_bad_page(p.err, kBadAttend, it.b);
+        report_bad_page(p.err, kBadAttend, b);
         return kNoRow;
       }
       return ((unsigned)pg * (unsigned)p.hk + kvh) * (unsigned)p.page_size + (key - col * (unsigned)p.page_size);
     };
-    Chunk<KIND> kf[2][KC], vf[4][VC];
+    // Keys without a row load row 0 of the pages instead: S is masked, V set to zero where a tile has such keys.
+    constexpr int EB = Q8 ? 1 : 2;
+    Chunk<KIND> kf[TPI][2][KC], vf[TPI][4][VC];
     uint32_t ks = 127, vs = 127;  // scale bytes of this lane's key
     auto load_k = [&](uint32_t row) {
-      const uint32_t ra = __shfl_sync(0xffffffffu, row, r), rb = __shfl_sync(0xffffffffu, row, r + 8);
 #pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        kf[0][j].load(p.kp, ra, p.d, 32 * j + 8 * c);
-        kf[1][j].load(p.kp, rb, p.d, 32 * j + 8 * c);
-      }
-      if constexpr (Q8) ks = row != kNoRow ? p.ks[row] : 127;
+      for (int t = 0; t < TPI; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t from = __shfl_sync(0xffffffffu, row == kNoRow ? 0 : row, 16 * t + 8 * k + r);
+          const uint8_t *at = static_cast<const uint8_t *>(p.kp) + ((size_t)from * p.d + 8 * c) * EB;
+#pragma unroll
+          for (int j = 0; j < KC; ++j) kf[t][k][j].load(at + 32 * EB * j, 32 * j + 8 * c < p.d);
+        }
+      if constexpr (Q8) ks = p.ks[row == kNoRow ? 0 : row];
     };
     auto load_v = [&](uint32_t row) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t rk = __shfl_sync(0xffffffffu, row, 2 * c + (k & 1) + (k >> 1) * 8);
+      for (int t = 0; t < TPI; ++t)
 #pragma unroll
-        for (int j = 0; j < VC; ++j) vf[k][j].load(p.vp, rk, p.dv, 64 * j + 8 * r);
-      }
-      if constexpr (Q8) vs = row != kNoRow ? p.vs[row] : 127;
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t from = __shfl_sync(0xffffffffu, row == kNoRow ? 0 : row, 16 * t + 2 * c + (k & 1) + (k >> 1) * 8);
+          const uint8_t *at = static_cast<const uint8_t *>(p.vp) + ((size_t)from * p.dv + 8 * r) * EB;
+#pragma unroll
+          for (int j = 0; j < VC; ++j) vf[t][k][j].load(at + 64 * EB * j, 64 * j + 8 * r < p.dv);
+        }
+      if constexpr (Q8) vs = p.vs[row == kNoRow ? 0 : row];
     };
+#pragma unroll
+    for (int t = 0; t < TPI; ++t) {
+#pragma unroll
+      for (int j = 0; j < KC; ++j) kf[t][0][j].zero(), kf[t][1][j].zero();
+#pragma unroll
+      for (int j = 0; j < VC; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vf[t][k][j].zero();
+    }
 
-    unsigned k0 = (unsigned)(it.chunk * kChunk) + warp * 16;
-    uint32_t row = row_at(k0), next = row_at(k0 + 16 * WARPS);
+    unsigned k0 = (unsigned)t0 * (unsigned)p.tile;
+    uint32_t row = row_at(k0), next = row_at(k0 + KEYS);
     load_k(row);
     load_v(row);
 
@@ -434,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool live = n * 8 + r < nq;
-      const long long base = it.b * p.qs[0] + (h0 + n * 8 + r) * p.qs[1];
+      const long long base = b * p.qs[0] + (h0 + n * 8 + r) * p.qs[1];
       if constexpr (!Q8) {
 #pragma unroll
         for (int j = 0; j < KC; ++j)
@@ -487,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) m[n][i] = mo[n][i] = -INFINITY, l[n][i] = 0.0f;
+      for (int i = 0; i < 2; ++i) m[n][i] = mo[n][i] = kNoRef, l[n][i] = 0.0f;
 #pragma unroll
       for (int j = 0; j < VC; ++j)
 #pragma unroll
@@ -496,46 +626,68 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
           for (int e = 0; e < 4; ++e) o[n][j][i][e] = 0.0f;
     }
 
-    for (; k0 < end; k0 += 16 * WARPS) {
-      // S^T: s[n][0..1] key r, heads 2c, 2c + 1; s[n][2..3] key r + 8.
-      float s[NT][4];
+    for (; k0 < end; k0 += KEYS) {
+      // S^T: s[t][n][0..1] key 16 t + r, heads 2c, 2c + 1; s[t][n][2..3] key 16 t + r + 8.
+      float s[TPI][NT][4], ev[TPI][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int t = 0; t < TPI; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < KC; ++j)
+          for (int e = 0; e < 4; ++e) s[t][n][e] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const uint32_t a0 = kf[0][j].pair(i), a1 = kf[1][j].pair(i), a2 = kf[0][j].pair(i + 1), a3 = kf[1][j].pair(i + 1);
+        for (int j = 0; j < KC; ++j) {
+          uint32_t x[4], y[4];
+          kf[t][0][j].pairs(x);
+          kf[t][1][j].pairs(y);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int q = 0; q < QS; ++q) mma<BF>(s[t][n], x[i], y[i], x[i + 1], y[i + 1], qf[n][q][j][i], qf[n][q][j][i + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int from = 16 * t + r + 8 * k;
+          const bool see = __shfl_sync(0xffffffffu, row, from) != kNoRow;
+          float fk = 1.0f;
+          ev[t][k] = 0.0f;
+          if constexpr (Q8) {
+            fk = scale_value(__shfl_sync(0xffffffffu, ks, from));
+            ev[t][k] = (float)((int)__shfl_sync(0xffffffffu, vs, from) - 127);
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int q = 0; q < QS; ++q) mma<BF>(s[n], a0, a1, a2, a3, qf[n][q][j][i], qf[n][q][j][i + 1]);
+            for (int i = 0; i < 2; ++i) s[t][n][2 * k + i] = see ? s[t][n][2 * k + i] * (qscale[n][i] * fk) : -INFINITY;
         }
-      const bool see[2] = {__shfl_sync(0xffffffffu, row, r) != kNoRow, __shfl_sync(0xffffffffu, row, r + 8) != kNoRow};
-      float fk[2] = {1.0f, 1.0f}, ev[2] = {0.0f, 0.0f};
-      if constexpr (Q8) {
-        fk[0] = scale_value(__shfl_sync(0xffffffffu, ks, r)), fk[1] = scale_value(__shfl_sync(0xffffffffu, ks, r + 8));
-        ev[0] = (float)((int)__shfl_sync(0xffffffffu, vs, r) - 127), ev[1] = (float)((int)__shfl_sync(0xffffffffu, vs, r + 8) - 127);
       }
       load_k(next);
 
       bool raise = false;
       float top[NT][2], otop[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = see[e >> 1] ? s[n][e] * (qscale[n][e & 1] * fk[e >> 1]) : -INFINITY;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          top[n][i] = fmaxf(s[n][i], s[n][2 + i]);
-          raise |= top[n][i] > m[n][i] + kSlack;
-          if constexpr (Q8) {
-            otop[n][i] = fmaxf(s[n][i] + ev[0], s[n][2 + i] + ev[1]);
-            raise |= otop[n][i] > mo[n][i] + kSlack;
+          top[n][i] = otop[n][i] = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < TPI; ++t) {
+            top[n][i] = fmaxf(top[n][i], fmaxf(s[t][n][i], s[t][n][2 + i]));
+            if constexpr (Q8) otop[n][i] = fmaxf(otop[n][i], fmaxf(s[t][n][i] + ev[t][0], s[t][n][2 + i] + ev[t][1]));
           }
+          raise |= top[n][i] > m[n][i] + kSlack;
+          if constexpr (Q8) raise |= otop[n][i] > mo[n][i] + kSlack;
         }
+      if (!__all_sync(0xffffffffu, row != kNoRow)) {  // the last tile of a sequence, or a bad page
+#pragma unroll
+        for (int t = 0; t < TPI; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (__shfl_sync(0xffffffffu, row, 16 * t + 2 * c + (k & 1) + (k >> 1) * 8) == kNoRow)
+#pragma unroll
+              for (int j = 0; j < VC; ++j) vf[t][k][j].zero();
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -545,14 +697,14 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], k));
             const float up = fmaxf(m[n][i], top[n][i] - kHead);
-            l[n][i] *= guard_exp2(m[n][i], up);
-            float keep = guard_exp2(m[n][i], up);
+            float keep = ex2(m[n][i] - up);
+            l[n][i] *= keep;
             m[n][i] = up;
             if constexpr (Q8) {
 #pragma unroll
               for (int k = 4; k < 32; k <<= 1) otop[n][i] = fmaxf(otop[n][i], __shfl_xor_sync(0xffffffffu, otop[n][i], k));
               const float oup = fmaxf(mo[n][i], otop[n][i] - kHead);
-              keep = guard_exp2(mo[n][i], oup);
+              keep = ex2(mo[n][i] - oup);
               mo[n][i] = oup;
             }
 #pragma unroll
@@ -561,46 +713,48 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
               for (int e = 0; e < 4; ++e) o[n][j][e][i] *= keep, o[n][j][e][2 + i] *= keep;
           }
       }
-      // P^T: b0 keys 2c, 2c + 1 and b1 keys 2c + 8, 2c + 9 of head r, as two numbers each.
-      uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+      for (int t = 0; t < TPI; ++t) {
+        // P^T: b0 keys 2c, 2c + 1 and b1 keys 2c + 8, 2c + 9 of head r, as two numbers each.
+        uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = guard_exp2(s[n][e], m[n][e & 1]);
-          l[n][e & 1] += w[e];
-          if constexpr (Q8) w[e] = guard_exp2(s[n][e], mo[n][e & 1] - ev[e >> 1]);
-        }
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t h = BF ? f32_to_bf16x2(w[2 * k], w[2 * k + 1]) : f32_to_f16x2(w[2 * k], w[2 * k + 1]);
-          const float2 f = BF ? bf16x2_to_f32(h) : f16x2_to_f32(h);
-          const float x = w[2 * k] - f.x, y = w[2 * k + 1] - f.y;
-          hi[n][k] = transpose8x8(h);
-          lo[n][k] = transpose8x8(BF ? f32_to_bf16x2(x, y) : f32_to_f16x2(x, y));
-        }
-      }
+          for (int e = 0; e < 4; ++e) {
+            w[e] = ex2(s[t][n][e] - m[n][e & 1]);
+            l[n][e & 1] += w[e];
+            if constexpr (Q8) w[e] = ex2(s[t][n][e] - (mo[n][e & 1] - ev[t][e >> 1]));
+          }
 #pragma unroll
-      for (int j = 0; j < VC; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t a0, a1, a2, a3;
-          key_pairs<KIND>(vf[0][j], vf[1][j], i, a0, a1);
-          key_pairs<KIND>(vf[2][j], vf[3][j], i, a2, a3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma<BF>(o[n][j][i], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-            mma<BF>(o[n][j][i], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t h = BF ? f32_to_bf16x2(w[2 * k], w[2 * k + 1]) : f32_to_f16x2(w[2 * k], w[2 * k + 1]);
+            const float2 f = BF ? bf16x2_to_f32(h) : f16x2_to_f32(h);
+            const float x = w[2 * k] - f.x, y = w[2 * k + 1] - f.y;
+            hi[n][k] = transpose8x8(h);
+            lo[n][k] = transpose8x8(BF ? f32_to_bf16x2(x, y) : f32_to_f16x2(x, y));
           }
         }
+#pragma unroll
+        for (int j = 0; j < VC; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t a0, a1, a2, a3;
+            key_pairs<KIND>(vf[t][0][j], vf[t][1][j], i, a0, a1);
+            key_pairs<KIND>(vf[t][2][j], vf[t][3][j], i, a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma<BF>(o[n][j][i], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+              if constexpr (LO) mma<BF>(o[n][j][i], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+            }
+          }
+      }
       load_v(next);
       row = next;
-      next = row_at(k0 + 2 * 16 * WARPS);
+      next = row_at(k0 + 2 * KEYS);
     }
 
-    // The warps meet in shared memory. o[n][j][i]: columns 64 j + 8 r + 2 i (e < 2) and + 1, heads 2c, 2c + 1.
-    __syncthreads();  // the last item's shared arrays are free
+    // o[n][j][i]: columns 64 j + 8 r + 2 i (e < 2) and + 1, heads 2c, 2c + 1.
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -615,80 +769,99 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : 3) mma_ke
           for (int e = 0; e < 4; ++e)
             *reinterpret_cast<float2 *>(&so[warp][q][64 * j + 8 * r + 2 * e]) = make_float2(o[n][j][e][i], o[n][j][e][2 + i]);
       }
-    __syncthreads();
-    const bool whole = it.chunk == 0 && c1 == it.chunks;
-    for (int i = threadIdx.x; i < nq * DP; i += kThreads) {
-      const int q = i / DP, e = i % DP;
-      float top = -INFINITY, otop = -INFINITY, sum = 0.0f, v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sml[w][q][0]), otop = fmaxf(otop, sml[w][q][1]);
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        sum = fmaf(sml[w][q][2], guard_exp2(sml[w][q][0], top), sum);
-        v = fmaf(so[w][q][e], guard_exp2(sml[w][q][1], otop), v);
-      }
-      if (whole) {
-        if (e < p.dv)
-          store_f32(p.out, p.dt, it.b * p.os[0] + (h0 + q) * p.os[1] + e, sum != 0.0f ? v * exp2f(otop - top) / sum : 0.0f);
-        if (p.lse && e == 0) p.lse[(long long)it.b * p.H + h0 + q] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
-      } else {
-        float *ws = slot(p, blockIdx.x, it.chunk == 0, q);
-        if (e < p.dv) ws[4 + e] = v;
-        if (e == 0) ws[0] = top, ws[1] = otop, ws[2] = sum;
-      }
-    }
-    g += c1 - it.chunk;
-    it.chunk = 0;
-    if (++it.head == p.hk * p.qt) {
-      it.head = 0;
-      if (g < run.g1)
-        do it.chunks = chunks_of(p, ++it.b);
-        while (it.chunks == 0);
-    }
-  }
+  });
 }
 
 // ---- join -----------------------------------------------------------------------------------------
-// Block (i, q) joins the item that starts in CTA i and ends in a later one, query q of its tile.
-__global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int ctas) {
-  __shared__ long long sm[kThreads / 32], found[2];
-  const int cta = blockIdx.x, q = blockIdx.y;
-  const Run run = run_of(p, cta, ctas, sm);
-  if (run.g0 >= run.g1) return;
-  const Item it = item_of(p, run.g1 - 1, sm, found);
-  const long long start = run.g1 - 1 - it.chunk, end = start + it.chunks;
-  if (start < run.g0 || end <= run.g1) return;
-  const int kvh = it.head / p.qt, h = kvh * p.group + (it.head % p.qt) * p.gt + q;
-  if (h >= (kvh + 1) * p.group) return;
-  const int last = (int)((end * run.n - 1) / run.total);  // the CTA of chunk end - 1
-  float top = -INFINITY, otop = -INFINITY, sum = 0.0f;
-  for (int c = cta; c <= last; ++c) {
-    const float *ws = slot(p, c, c == cta, q);
-    top = fmaxf(top, ws[0]);
-    otop = fmaxf(otop, ws[1]);
-  }
-  for (int c = cta; c <= last; ++c) {
-    const float *ws = slot(p, c, c == cta, q);
-    sum = fmaf(ws[2], guard_exp2(ws[0], top), sum);
-  }
-  for (int e = threadIdx.x; e < p.dv; e += kThreads) {
-    float v = 0.0f;
-    for (int c = cta; c <= last; ++c) {
-      const float *ws = slot(p, c, c == cta, q);
-      v = fmaf(ws[4 + e], guard_exp2(ws[1], otop), v);
+// Block (i, q) joins query q of the items that the warps of block i start and later ones end: one such item
+// is shared by the block's warps, each taking every fourth part; of several, a warp has one each. Lanes hold
+// the parts' headers, then each lane columns of O, of the parts that have any weight.
+__global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
+  __shared__ float so[kWarps][1][256];
+  __shared__ float sml[kWarps][1][3];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = blockIdx.y;
+  int mine = -1, owners = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if (p.owners[blockIdx.x * kWarps + w].z >= 0) {
+      ++owners;
+      if (mine < 0 || w == warp) mine = w;
     }
-    v = sum != 0.0f ? v * exp2f(otop - top) / sum : 0.0f;
-    store_f32(p.out, p.dt, it.b * p.os[0] + h * p.os[1] + e, v);
+  if (!owners) return;
+  const bool meet = owners == 1;
+  const int first = blockIdx.x * kWarps + (meet ? mine : warp);
+  const int4 own = p.owners[first];
+  if (own.z < 0) return;
+  const int kvh = own.y / p.qt, h = kvh * p.group + (own.y % p.qt) * p.gt + q;
+  if (h >= (kvh + 1) * p.group) return;
+  const int step = meet ? kWarps : 1, at0 = meet ? warp : 0;
+  const int parts = (own.z - first + step - at0) / step;  // this warp's: first + at0, + step, ..
+  auto part = [&](int i) { return slot(p, first + at0 + i * step, at0 + i == 0, q); };
+  float top = -INFINITY, otop = -INFINITY;
+  for (int i = lane; i < parts; i += 32) {
+    const float4 x = *reinterpret_cast<const float4 *>(part(i));
+    top = fmaxf(top, x.x), otop = fmaxf(otop, x.y);
   }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[(long long)it.b * p.H + h] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+#pragma unroll
+  for (int k = 16; k; k >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    otop = fmaxf(otop, __shfl_xor_sync(0xffffffffu, otop, k));
+  }
+  float sum = 0.0f, v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    float4 x = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+    if (i0 + lane < parts) x = *reinterpret_cast<const float4 *>(part(i0 + lane));
+    float l = x.z * guard_exp2(x.x, top);
+    const float f = guard_exp2(x.y, otop);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    sum += l;
+    unsigned live = __ballot_sync(0xffffffffu, f != 0.0f);
+    while (live) {  // four parts' loads in flight
+      const float *y[4];
+      float w[4], z[4][8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = live ? __ffs(live) - 1 : 0;
+        w[k] = __shfl_sync(0xffffffffu, f, i);
+        if (!live) w[k] = 0.0f;
+        live &= live - 1;
+        y[k] = part(i0 + i) + 4;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[k][e] = lane + 32 * e < p.dv && w[k] != 0.0f ? y[k][lane + 32 * e] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(z[k][e], w[k], v[e]);
+    }
+  }
+  if (!meet) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (lane + 32 * e < p.dv) put(p, own.x, h, lane + 32 * e, v[e], sum, top, otop);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) so[warp][0][lane + 32 * e] = v[e];
+  if (lane == 0) sml[warp][0][0] = top, sml[warp][0][1] = otop, sml[warp][0][2] = sum;
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.dv; e += kThreads) {
+    combine<kWarps>(so, sml, 0, e, v[0], sum, top, otop);
+    put(p, own.x, h, e, v[0], sum, top, otop);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------
 struct Plan {
-  int gt, qt, ctas;
+  int gt, qt, ctas, tile;
   int dp;  // padded head dim of the tensor-core kernel, 0: the CUDA cores
-  size_t ws_bytes;
+  size_t owners_bytes, ws_bytes;
 };
 
 static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_desc *d, bool aligned, Plan *pl) {
@@ -708,20 +881,27 @@ static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_d
     if (s < 0) return fail(MPC_ERR_INVALID, "mpc_sdpa_paged: negative stride");
   const int64_t group = d->h / c->hk, dm = c->d > c->dv ? c->d : c->dv;
   // The tensor cores take rows of 16 and 8 bits in aligned pieces of 8 values, their numbers in 32 bits.
-  const bool tc = aligned && c->dtype != MPC_F32 && c->d % 8 == 0 && c->dv % 8 == 0 &&
+  const bool tc = aligned && c->dtype != MPC_F32 && c->n_pages > 0 && c->d % 8 == 0 && c->dv % 8 == 0 &&
                   c->n_pages * c->page_size < (int64_t)kNoRow / c->hk;
   const bool two = c->dtype == MPC_E4M3 && d->dtype == MPC_F32;  // two f16 per query value: no registers for 16 heads
   pl->dp = !tc ? 0 : dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
   pl->gt = tc ? (group > 8 && pl->dp < 256 && !two ? 16 : 8) : group >= 4 ? 4 : group >= 2 ? 2 : 1;
   pl->qt = (int)((group + pl->gt - 1) / pl->gt);
-  // As many CTAs as are resident, fewer where even the longest lengths give fewer chunks.
-  const long long per = (d->max_pages * c->page_size + kChunk - 1) / kChunk;
-  const long long sms = (long long)dev->prop.multiProcessorCount * (tc && (pl->dp == 256 || pl->gt == 16) ? 2 : 3);
+  pl->tile = !tc ? 16 : pl->dp == 64 ? 16 * D64_TPI : pl->dp == 128 && c->dtype == MPC_E4M3 ? 16 * E4_TPI : 16;
+  // Fewer than 2^31 units (and half of that for the sums of their parts), by longer tiles where a table could hold more.
+  while ((double)d->b * c->hk * pl->qt * (double)(d->max_pages * c->page_size / pl->tile + 1 + kItemCost) >= (double)(1 << 30)) {
+    if (pl->tile >= (1 << 30)) return fail(MPC_ERR_UNSUPPORTED, "mpc_sdpa_paged: too many sequences and heads");
+    pl->tile *= 2;
+  }
+  // As many CTAs as are resident, fewer where even the longest lengths give fewer tiles than warps.
+  const long long per = (d->max_pages * c->page_size + kWarps * pl->tile - 1) / (kWarps * pl->tile);
+  const long long sms = (long long)dev->prop.multiProcessorCount * (!tc ? 3 : pl->dp == 256 || pl->gt == 16 ? 2 : pl->dp == 64 ? D64_MINB : c->dtype == MPC_E4M3 ? E4_MINB : 3);
   const long long heads = c->hk * pl->qt;
   long long ctas = sms;
   if (d->b > 0 && per > 0 && per <= sms / heads / d->b) ctas = per * heads * d->b;
   pl->ctas = (int)(ctas < 1 ? 1 : ctas);
-  pl->ws_bytes = (size_t)pl->ctas * 2 * pl->gt * (c->dv + 4) * sizeof(float);
+  pl->owners_bytes = (size_t)pl->ctas * kWarps * sizeof(int4);
+  pl->ws_bytes = pl->owners_bytes + (size_t)pl->ctas * kWarps * 2 * pl->gt * slot_floats((int)c->dv) * sizeof(float);
   return MPC_OK;
 }
 
@@ -732,13 +912,13 @@ static void launch_simt(const Params &p, int ctas, cudaStream_t st) {
   else simt_kernel<NI, 1, VEC><<<ctas, kThreads, 0, st>>>(p);
 }
 
-template <int KIND, int QS>
+template <int KIND, int QS, bool LO>
 static void launch_mma(const Params &p, const Plan &pl, cudaStream_t st) {
   constexpr int NT = QS == 2 ? 1 : 2;
   auto run = [&](auto kern) { kern<<<pl.ctas, kThreads, 0, st>>>(p); };
-  if (pl.dp == 64) pl.gt == 16 ? run(mma_kernel<KIND, 64, NT, QS>) : run(mma_kernel<KIND, 64, 1, QS>);
-  else if (pl.dp == 128) pl.gt == 16 ? run(mma_kernel<KIND, 128, NT, QS>) : run(mma_kernel<KIND, 128, 1, QS>);
-  else run(mma_kernel<KIND, 256, 1, QS>);
+  if (pl.dp == 64) pl.gt == 16 ? run(mma_kernel<KIND, 64, NT, QS, LO>) : run(mma_kernel<KIND, 64, 1, QS, LO>);
+  else if (pl.dp == 128) pl.gt == 16 ? run(mma_kernel<KIND, 128, NT, QS, LO>) : run(mma_kernel<KIND, 128, 1, QS, LO>);
+  else run(mma_kernel<KIND, 256, 1, QS, LO>);
 }
 
 }  // namespace paged
@@ -789,26 +969,39 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
   }
   Params p{};
   p.q = Q, p.kp = k_pages, p.vp = v_pages, p.ks = k_scale, p.vs = v_scale, p.table = table, p.lengths = lengths;
-  p.out = O, p.lse = LSE, p.ws = static_cast<float *>(workspace), p.err = dev->d_err;
+  p.out = O, p.lse = LSE, p.err = dev->d_err, p.tile = pl.tile, p.owners = static_cast<int4 *>(workspace);
+  p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + pl.owners_bytes);
   for (int i = 0; i < 2; ++i) p.qs[i] = desc->q_stride[i], p.os[i] = desc->o_stride[i];
   p.max_pages = desc->max_pages, p.cap = desc->max_pages * cache->page_size;
   p.B = (int)desc->b, p.H = (int)desc->h, p.hk = (int)cache->hk, p.group = p.H / p.hk, p.gt = pl.gt, p.qt = pl.qt;
   p.d = (int)cache->d, p.dv = (int)cache->dv, p.page_size = (int)cache->page_size, p.n_pages = (int)cache->n_pages;
+  // With 2^(l-1) < page_size <= 2^l and page_mul = ceil(2^(31+l) / page_size) (below 2^32), page_mul * page_size exceeds
+  // 2^(31+l) by less than 2^l, so the quotient is exact for keys below 2^31.
+  int l = 0;
+  while ((1 << l) < p.page_size) ++l;
+  p.page_shift = 31 + l, p.page_mul = (uint32_t)(((1ull << (31 + l)) + p.page_size - 1) / p.page_size);
   p.dt = desc->dtype, p.dt_pages = cache->dtype, p.scale_log2 = desc->scale * kLog2e;
   const bool vec = aligned && p.d % 8 == 0 && p.dv % 8 == 0;
   const int dm = p.d > p.dv ? p.d : p.dv;
-  if (pl.dp && cache->dtype == MPC_F16) launch_mma<kF16, 1>(p, pl, st);
-  else if (pl.dp && cache->dtype == MPC_BF16) launch_mma<kBF16, 1>(p, pl, st);
-  else if (pl.dp && desc->dtype == MPC_F32) launch_mma<kE4M3, 2>(p, pl, st);
-  else if (pl.dp) launch_mma<kE4M3, 1>(p, pl, st);
+  if (pl.dp && cache->dtype == MPC_F16) launch_mma<kF16, 1, true>(p, pl, st);
+  else if (pl.dp && cache->dtype == MPC_BF16) launch_mma<kBF16, 1, true>(p, pl, st);
+  else if (pl.dp && desc->dtype == MPC_F32) launch_mma<kE4M3, 2, true>(p, pl, st);
+  else if (pl.dp && desc->dtype == MPC_F16) launch_mma<kE4M3, 1, true>(p, pl, st);
+  else if (pl.dp) launch_mma<kE4M3, 1, false>(p, pl, st);
   else if (dm <= 64) vec ? launch_simt<1, true>(p, pl.ctas, st) : launch_simt<1, false>(p, pl.ctas, st);
   else if (dm <= 128) vec ? launch_simt<2, true>(p, pl.ctas, st) : launch_simt<2, false>(p, pl.ctas, st);
   else vec ? launch_simt<4, true>(p, pl.ctas, st) : launch_simt<4, false>(p, pl.ctas, st);
   dev->launches++;
   if ((rc = check_launch(dev, "mpc_sdpa_paged"))) return rc;
-  join_kernel<<<dim3(pl.ctas, pl.gt), kThreads, 0, st>>>(p, pl.ctas);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pl.ctas, p.group < pl.gt ? p.group : pl.gt), cfg.blockDim = dim3(kThreads), cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  MPC_CUDA(dev, cudaLaunchKernelEx(&cfg, join_kernel, p));
   dev->launches++;
-  return check_launch(dev, "mpc_sdpa_paged join");
+  return MPC_OK;
 }
 
 }  // extern "C"
