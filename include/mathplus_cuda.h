@@ -346,8 +346,8 @@ int mpc_kv_read(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, 
  * LSE -inf; rows behind a sequence's length are never used, whatever they hold. Q [b, h, d] and O
  * [b, h, dv] have element strides (sequence, head) and a contiguous last axis; their dtype is the cache's,
  * or any float type over MPC_E4M3. LSE (optional, f32 [b, h]) is the natural-log normaliser. The work is
- * split along the cache by the lengths found on the device and joined by a second small kernel; the
- * partial results live in the workspace. A length that is negative or beyond max_pages * page_size, or a
+ * split along the cache by the lengths found on the device; the partial results live in the workspace
+ * until the block that completes an item joins them. A length that is negative or beyond max_pages * page_size, or a
  * page outside the cache, is cut off or left out, and the next synchronisation returns MPC_ERR_INVALID. */
 typedef struct {
   int64_t b, h, max_pages;
@@ -358,8 +358,9 @@ typedef struct {
 /* Bytes that mpc_sdpa_paged needs as workspace for any lengths within the table. */
 int mpc_sdpa_paged_workspace(mpc_device *dev, const mpc_kv_desc *cache, const mpc_sdpa_paged_desc *desc, size_t *bytes);
 /* workspace NULL: taken from the device's allocator for this call (not while s is being captured into a
- * graph). A workspace given must not be used by another call at the same time; graphs that may run side
- * by side need one each. 16-byte aligned. */
+ * graph). A workspace given is 16-byte aligned, zeroed before its first call and left ready for the next
+ * one of any shape that it is large enough for; it must not be used by two calls at the same time, so
+ * graphs that may run side by side need one each. */
 int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, const void *v_pages,
                    const uint8_t *k_scale, const uint8_t *v_scale, const mpc_sdpa_paged_desc *desc, const void *Q,
                    const int32_t *table, const int32_t *lengths, void *O, float *LSE, void *workspace,

@@ -41,6 +41,7 @@ struct mpc_device {
   int ordinal = -1;
   cudaStream_t stream = nullptr;
   int *d_err = nullptr;  // kernel error word (device memory)
+  int *d_counters = nullptr;  // zero between the kernels of `stream` that count in them
   std::atomic<int> sticky{0};
   uint64_t timeout_ns = 2000000000ull;
   std::atomic<uint64_t> launches{0};
@@ -57,6 +58,8 @@ struct mpc_comm {
 };
 
 namespace mpc {
+
+constexpr size_t kCounterBytes = 16384;  // of mpc_device::d_counters
 
 // Thread-local last-error text and the helpers that fill it.
 void set_error(const char *fmt, ...);

@@ -259,8 +259,12 @@ int mpc_device_create(int ordinal, unsigned flags, mpc_device **out) {
     return rc;
   }
   if ((e = cudaStreamCreateWithFlags(&dev->stream, cudaStreamNonBlocking)) != cudaSuccess ||
-      (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess || (e = cudaMemset(dev->d_err, 0, 256)) != cudaSuccess) {
+      (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess || (e = cudaMemset(dev->d_err, 0, 256)) != cudaSuccess ||
+      (e = cudaMalloc(&dev->d_counters, kCounterBytes)) != cudaSuccess ||
+      (e = cudaMemset(dev->d_counters, 0, kCounterBytes)) != cudaSuccess) {
     rc = cuda_fail(nullptr, e, "mpc_device_create");
+    if (dev->d_err) cudaFree(dev->d_err);
+    if (dev->d_counters) cudaFree(dev->d_counters);
     if (dev->stream) cudaStreamDestroy(dev->stream);
     delete dev;
     return rc;
@@ -282,6 +286,7 @@ int mpc_device_destroy(mpc_device *dev) {
     for (auto &kv : dev->alloc.live) cudaFree(kv.first);
   }
   if (dev->d_err) cudaFree(dev->d_err);
+  if (dev->d_counters) cudaFree(dev->d_counters);
   if (dev->stream) cudaStreamDestroy(dev->stream);
   delete dev;
   return MPC_OK;

@@ -11,8 +11,9 @@
 // T (i + 1) / n). The runs are found from the lengths on the device, so ragged batches and a single long
 // sequence balance alike and the launch depends on host-known sizes alone (it can be captured into a
 // graph). A warp that has an item wholly writes the output. Otherwise the (at most two) cut items of
-// a warp leave (m, l, O) in the workspace, one for the block where all its warps are inside one item, and a
-// second kernel joins them in order, so the result does not depend on timing.
+// a warp leave (m, l, O) in the workspace, one for the block where all its warps are inside one item, and
+// count themselves there; the block that counts an item's last part joins them all, in their order, so the
+// result does not depend on timing. The counters are zero between calls: who joins puts them back.
 //
 // CUDA-core kernel (f32 rows, and any head dim <= 256 or alignment): 8 lanes per key, 4 keys at a time, each
 // group of 8 lanes with its own running maximum, sum and O, which meet once per item.
@@ -20,20 +21,16 @@
 
 #include "kv_cache.cuh"
 #include "mpc_internal.h"
-#include "sm100.cuh"
 
 namespace mpc {
 namespace paged {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-#ifndef ITEM_COST
-#define ITEM_COST 3
-#define E4_TPI 2
-#define E4_MINB 2
-#define D64_TPI 2
-#define D64_MINB 3
-#endif
-constexpr int kItemCost = ITEM_COST;
+constexpr int kMaxCtas = 4;  // resident on an SM, at most
+// Measured (GPU time; 0, 4, 8, 12, 24 tiles an item): 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 35, 28, 27,
+// 28, 33 us; 32 sequences of 500..8191 keys, 8 heads of 128, f16: 109, 100, 98, 98, 99 us; 2 of ~115k keys in 8 bits:
+// 103, 95, 91, 90, 92 us.
+constexpr int kItemCost = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -42,12 +39,13 @@ struct Params {
   const int32_t *table, *lengths;
   void *out;
   float *lse, *ws;
-  int4 *owners;  // per warp: (sequence, head tile, last warp, unused) of the item it starts and another ends; last -1: none
+  int *counters;  // per warp: the warps that have left their part of the item that it starts
   int *err;
   long long qs[2], os[2], max_pages, cap;  // cap: max_pages * page_size
   int B, H, hk, group, gt, qt, tile;  // query heads per K/V head, per query tile; tiles per K/V head; keys of a tile
   int d, dv, page_size, n_pages, dt, dt_pages;
   uint32_t page_mul, page_shift;  // key / page_size = key * page_mul >> page_shift for keys below 2^31
+  int q_vec;  // queries in aligned pieces of 8 values
   float scale_log2;
   __device__ __forceinline__ unsigned page_of(unsigned key) const { return (unsigned)((uint64_t)key * page_mul >> page_shift); }
 };
@@ -212,6 +210,84 @@ __device__ __forceinline__ void finish(const Params &p, const Item &it, int t0, 
   }
 }
 
+// An item whose parts are all in the workspace: those of warps first..last.
+struct Join {
+  Item it;
+  int first, last;
+};
+
+// Whether a block's run is inside one item, so that its warps leave one part, in its first warp's place.
+__device__ __forceinline__ bool meets(const Deal &all, const Item &it, int block) {
+  const int w0 = block * kWarps;
+  return all.start(w0) >= it.start && all.start(min(w0 + kWarps, all.n)) <= it.start + it.units;
+}
+
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+
+// Counts `warps` more warps' part of a cut item (the caller has fenced its stores); true for the last part.
+__device__ __forceinline__ bool last_part(const Params &p, const Deal &all, const Item &it, int warps, Join &j) {
+  const int wf = all.warp_of(it.start + kItemCost);  // the warp of the first tile; warps before it have no part
+  j.it = it;
+  j.first = meets(all, it, wf / kWarps) ? wf / kWarps * kWarps : wf;
+  j.last = all.warp_of(it.start + it.units - 1);
+  if (atomicAdd(p.counters + j.first, warps) + warps != j.last - j.first + 1) return false;
+  p.counters[j.first] = 0;
+  fence_gpu();
+  return true;
+}
+
+// One warp joins query q of an item, eight parts' loads in flight: every lane reads a part's header and four or
+// eight columns of its O.
+__device__ __forceinline__ void join(const Params &p, const Deal &all, const Join &j, int q) {
+  const int lane = threadIdx.x & 31;
+  const int kvh = j.it.head / p.qt, h = kvh * p.group + (j.it.head % p.qt) * p.gt + q;
+  const bool in0 = 4 * lane < p.dv, in1 = 4 * lane + 128 < p.dv;
+  float top = -INFINITY, otop = -INFINITY, sum = 0.0f;
+  float4 v[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+  for (int w = j.first; w <= j.last;) {
+    float4 x[8], z[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x[k] = make_float4(-INFINITY, -INFINITY, 0, 0);
+      z[k][0] = z[k][1] = make_float4(0, 0, 0, 0);
+      if (w <= j.last) {
+        const float4 *y = reinterpret_cast<const float4 *>(slot(p, w, w == j.first, q));
+        x[k] = __ldcg(y);
+        if (in0) z[k][0] = __ldcg(y + 1 + lane);
+        if (in1) z[k][1] = __ldcg(y + 33 + lane);
+        w += w % kWarps == 0 && meets(all, j.it, w / kWarps) ? kWarps : 1;
+      }
+    }
+    float up = top, oup = otop;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) up = fmaxf(up, x[k].x), oup = fmaxf(oup, x[k].y);
+    sum *= guard_exp2(top, up);
+    const float keep = guard_exp2(otop, oup);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e].x *= keep, v[e].y *= keep, v[e].z *= keep, v[e].w *= keep;
+    top = up, otop = oup;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      sum = fmaf(x[k].z, guard_exp2(x[k].x, top), sum);
+      const float f = guard_exp2(x[k].y, otop);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[e].x = fmaf(z[k][e].x, f, v[e].x), v[e].y = fmaf(z[k][e].y, f, v[e].y);
+        v[e].z = fmaf(z[k][e].z, f, v[e].z), v[e].w = fmaf(z[k][e].w, f, v[e].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float y[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = 128 * e + 4 * lane + k;
+      if (at < p.dv) put(p, j.it.b, h, at, y[k], sum, top, otop);
+    }
+  }
+}
+
 // Walks a warp's run: body(sequence, head tile, t0, t1) leaves its part of each item in shared memory. The place
 // in the run is in shared memory too, while the body has the registers.
 template <int GT, int PITCH, typename Body>
@@ -223,16 +299,20 @@ __device__ __forceinline__ void walk(const Params &p, float (*so)[GT][PITCH], fl
   __shared__ int sm[kWarps + 2];
   __shared__ Place places[kWarps];
   __shared__ Deal all;
+  __shared__ Item cut[kWarps][2];  // a warp's run cuts two items at most
+  __shared__ Join joins[2 * kWarps];
+  __shared__ int n_joins;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gw = blockIdx.x * kWarps + warp;
   volatile Place *const here = &places[warp];
   bool meet = false;  // the block is inside one item: its warps meet at the end
   bool go = false;
+  int cuts = 0;
   {
     Deal deal;
     Item it{};
     int u0 = 0, u1 = 0;
     if (find_run(p, sm, deal, it)) {
-      meet = deal.start(min(gw - warp + kWarps, deal.n)) <= it.start + it.units;
+      meet = meets(deal, it, blockIdx.x);
       if (gw < deal.n) u0 = deal.start(gw), u1 = deal.start(gw + 1);
       go = u0 < u1 || meet;
       if (!meet && go)
@@ -240,42 +320,53 @@ __device__ __forceinline__ void walk(const Params &p, float (*so)[GT][PITCH], fl
     }
     if (lane == 0) {
       places[warp].it = it, places[warp].u = u0, places[warp].u1 = u1;
-      p.owners[gw] = make_int4(0, 0, -1, 0);
-      if (warp == 0) all = deal;
+      if (warp == 0) all = deal, n_joins = 0;
     }
   }
   __syncthreads();
-  grid_dependents_launch();  // every block is running by now: the join's blocks may take the places that become free
   while (go) {
     int u = here->u, end = min(here->u1, here->it.start + here->it.units), base = here->it.start + kItemCost;
     if (meet || end > base) body(here->it.b, here->it.head, max(0, u - base), max(0, end - base));
     __syncwarp();
     Item it;
     it.b = here->it.b, it.head = here->it.head, it.start = here->it.start, it.units = here->it.units;
-    const int u1 = here->u1;
+    const int u1 = here->u1, w0 = gw - warp;
     u = here->u, end = min(u1, it.start + it.units), base = it.start + kItemCost;
     int from = max(0, u - base), to = max(0, end - base);
     if (meet) {
       __syncthreads();
-      if (warp && lane < GT && u < u1)  // the block's part goes to its first warp's place
-        *reinterpret_cast<float4 *>(slot(p, gw, false, lane)) = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
-      const int w0 = gw - warp;
       from = max(0, all.start(w0) - base), to = max(0, all.start(min(w0 + kWarps, all.n)) - base);
       if (to > from) finish<kWarps, GT, PITCH>(p, it, from, to, w0, so, sml, threadIdx.x, kThreads);
+      __syncthreads();
     } else if (to > from) {
       finish<1, GT, PITCH>(p, it, from, to, gw, so + warp, sml + warp, lane, 32);
     }
-    if (lane == 0 && (!meet || warp == 0) && from == 0 && to > 0 && to < it.units - kItemCost)
-      p.owners[gw] = make_int4(it.b, it.head, all.warp_of(it.start + it.units - 1), 0);
-    go = !meet && end < u1;
     __syncwarp();
+    if ((!meet || warp == 0) && to > from && to - from < it.units - kItemCost) {
+      if (lane == 0) cut[warp][cuts] = it;
+      ++cuts;
+    }
+    go = !meet && end < u1;
     if (go) {
       advance(p, it);
       if (lane == 0) places[warp].it = it, places[warp].u = end;
       __syncwarp();
     }
   }
+  // The parts are counted once the run is done: one fence, and the two items' counters at once.
+  __syncwarp();
+  if (lane < cuts) {
+    fence_gpu();
+    Join j;
+    const int w0 = gw - warp;
+    if (last_part(p, all, cut[warp][lane], meet ? min(kWarps, all.n - w0) : 1, j)) joins[atomicAdd(&n_joins, 1)] = j;
+  }
   empty_rows(p);
+  __syncthreads();
+  for (int i = warp; i < n_joins * GT; i += kWarps) {
+    const Join j = joins[i / GT];
+    if (i % GT < p.group - (j.it.head % p.qt) * GT) join(p, all, j, i % GT);
+  }
 }
 
 // ---- CUDA-core kernel ---------------------------------------------------------------------------
@@ -485,12 +576,14 @@ __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND
 
 // DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value; LO: weights as two
 // numbers. TPI tiles of 16
-// keys at a time: 32 keys where their rows fit the registers that 16 longer ones take.
+// keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks per SM as the registers
+// allow; over 8-bit rows of 128 two blocks of 32 keys a warp (91 us at 2 x ~115k keys) beat three or four of 16 (100 us).
 template <int KIND, int DP>
-constexpr int tiles_at_once() { return DP == 64 ? D64_TPI : (DP == 128 && KIND == kE4M3) ? E4_TPI : 1; }
+constexpr int tiles_at_once() { return DP == 64 || (DP == 128 && KIND == kE4M3) ? 2 : 1; }
+constexpr int blocks_per_sm(bool e4m3, int dp, int heads) { return dp == 256 || heads == 16 || (dp == 128 && e4m3) ? 2 : 3; }
 
 template <int KIND, int DP, int NT, int QS, bool LO>
-__global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : DP == 64 ? D64_MINB : KIND == kE4M3 ? E4_MINB : 3) mma_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND == kE4M3, DP, 8 * NT)) mma_kernel(const Params p) {
   constexpr bool BF = KIND == kBF16, Q8 = KIND == kE4M3;
   constexpr int KC = DP / 32, VC = DP / 64, GT = 8 * NT, PITCH = DP + 8, TPI = tiles_at_once<KIND, DP>(), KEYS = 16 * TPI;
   __shared__ alignas(16) float so[kWarps][GT][PITCH];  // written as pairs
@@ -564,29 +657,36 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : DP == 64 
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool live = n * 8 + r < nq;
-      const long long base = b * p.qs[0] + (h0 + n * 8 + r) * p.qs[1];
+      const long long base = b * p.qs[0] + (h0 + n * 8 + r) * p.qs[1] + 8 * c;
       if constexpr (!Q8) {
 #pragma unroll
-        for (int j = 0; j < KC; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = 32 * j + 8 * c + 2 * i;
-            const uint16_t *q = static_cast<const uint16_t *>(p.q) + base + at;
-            qf[n][0][j][i] = live && at < p.d ? (uint32_t)q[0] | (uint32_t)q[1] << 16 : 0u;
+        for (int j = 0; j < KC; ++j) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (live && 32 * j + 8 * c < p.d) {
+            const uint16_t *q = static_cast<const uint16_t *>(p.q) + base + 32 * j;
+            if (p.q_vec) x = *reinterpret_cast<const uint4 *>(q);
+            else x = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
           }
+          qf[n][0][j][0] = x.x, qf[n][0][j][1] = x.y, qf[n][0][j][2] = x.z, qf[n][0][j][3] = x.w;
+        }
         qscale[n][0] = qscale[n][1] = p.scale_log2;
       } else {
+        float x[KC][8];
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < KC; ++j)
+        for (int j = 0; j < KC; ++j) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+          if (live && 32 * j + 8 * c < p.d) {
+            if (p.q_vec) load8<true>(p.q, p.dt, base + 32 * j, 8, x[j]);
+            else load8<false>(p.q, p.dt, base + 32 * j, 8, x[j]);
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int at = 32 * j + 8 * c + i;
-            if (live && at < p.d) {
-              const uint32_t a = __float_as_uint(load_f32(p.q, p.dt, base + at)) & 0x7fffffffu;
-              if (a < 0x7f800000u) top = max(top, a);
-            }
+            const uint32_t a = __float_as_uint(x[j][i]) & 0x7fffffffu;
+            if (a < 0x7f800000u) top = max(top, a);
           }
+        }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int eq = max(1, min((int)(top >> 23), 253)) - 127;  // the row's largest is in [2^eq, 2^(eq + 1))
@@ -597,9 +697,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : DP == 64 
         for (int j = 0; j < KC; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int at = 32 * j + 8 * c + 2 * i;
-            float x0 = 0.0f, x1 = 0.0f;
-            if (live && at < p.d) x0 = load_f32(p.q, p.dt, base + at) * f0 * f1, x1 = load_f32(p.q, p.dt, base + at + 1) * f0 * f1;
+            const float x0 = x[j][2 * i] * f0 * f1, x1 = x[j][2 * i + 1] * f0 * f1;
             qf[n][0][j][i] = f32_to_f16x2(x0, x1);
             if constexpr (QS == 2) {
               const float2 h = f16x2_to_f32(qf[n][0][j][i]);
@@ -772,96 +870,11 @@ __global__ void __launch_bounds__(kThreads, DP == 256 || NT == 2 ? 2 : DP == 64 
   });
 }
 
-// ---- join -----------------------------------------------------------------------------------------
-// Block (i, q) joins query q of the items that the warps of block i start and later ones end: one such item
-// is shared by the block's warps, each taking every fourth part; of several, a warp has one each. Lanes hold
-// the parts' headers, then each lane columns of O, of the parts that have any weight.
-__global__ void __launch_bounds__(kThreads) join_kernel(const Params p) {
-  __shared__ float so[kWarps][1][256];
-  __shared__ float sml[kWarps][1][3];
-  grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = blockIdx.y;
-  int mine = -1, owners = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w)
-    if (p.owners[blockIdx.x * kWarps + w].z >= 0) {
-      ++owners;
-      if (mine < 0 || w == warp) mine = w;
-    }
-  if (!owners) return;
-  const bool meet = owners == 1;
-  const int first = blockIdx.x * kWarps + (meet ? mine : warp);
-  const int4 own = p.owners[first];
-  if (own.z < 0) return;
-  const int kvh = own.y / p.qt, h = kvh * p.group + (own.y % p.qt) * p.gt + q;
-  if (h >= (kvh + 1) * p.group) return;
-  const int step = meet ? kWarps : 1, at0 = meet ? warp : 0;
-  const int parts = (own.z - first + step - at0) / step;  // this warp's: first + at0, + step, ..
-  auto part = [&](int i) { return slot(p, first + at0 + i * step, at0 + i == 0, q); };
-  float top = -INFINITY, otop = -INFINITY;
-  for (int i = lane; i < parts; i += 32) {
-    const float4 x = *reinterpret_cast<const float4 *>(part(i));
-    top = fmaxf(top, x.x), otop = fmaxf(otop, x.y);
-  }
-#pragma unroll
-  for (int k = 16; k; k >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    otop = fmaxf(otop, __shfl_xor_sync(0xffffffffu, otop, k));
-  }
-  float sum = 0.0f, v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    float4 x = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
-    if (i0 + lane < parts) x = *reinterpret_cast<const float4 *>(part(i0 + lane));
-    float l = x.z * guard_exp2(x.x, top);
-    const float f = guard_exp2(x.y, otop);
-#pragma unroll
-    for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-    sum += l;
-    unsigned live = __ballot_sync(0xffffffffu, f != 0.0f);
-    while (live) {  // four parts' loads in flight
-      const float *y[4];
-      float w[4], z[4][8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = live ? __ffs(live) - 1 : 0;
-        w[k] = __shfl_sync(0xffffffffu, f, i);
-        if (!live) w[k] = 0.0f;
-        live &= live - 1;
-        y[k] = part(i0 + i) + 4;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[k][e] = lane + 32 * e < p.dv && w[k] != 0.0f ? y[k][lane + 32 * e] : 0.0f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(z[k][e], w[k], v[e]);
-    }
-  }
-  if (!meet) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < p.dv) put(p, own.x, h, lane + 32 * e, v[e], sum, top, otop);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) so[warp][0][lane + 32 * e] = v[e];
-  if (lane == 0) sml[warp][0][0] = top, sml[warp][0][1] = otop, sml[warp][0][2] = sum;
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.dv; e += kThreads) {
-    combine<kWarps>(so, sml, 0, e, v[0], sum, top, otop);
-    put(p, own.x, h, e, v[0], sum, top, otop);
-  }
-}
-
 // ---- host -------------------------------------------------------------------------------------------
 struct Plan {
   int gt, qt, ctas, tile;
   int dp;  // padded head dim of the tensor-core kernel, 0: the CUDA cores
-  size_t owners_bytes, ws_bytes;
+  size_t counters_bytes, ws_bytes;
 };
 
 static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_desc *d, bool aligned, Plan *pl) {
@@ -887,7 +900,7 @@ static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_d
   pl->dp = !tc ? 0 : dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
   pl->gt = tc ? (group > 8 && pl->dp < 256 && !two ? 16 : 8) : group >= 4 ? 4 : group >= 2 ? 2 : 1;
   pl->qt = (int)((group + pl->gt - 1) / pl->gt);
-  pl->tile = !tc ? 16 : pl->dp == 64 ? 16 * D64_TPI : pl->dp == 128 && c->dtype == MPC_E4M3 ? 16 * E4_TPI : 16;
+  pl->tile = tc && (pl->dp == 64 || (pl->dp == 128 && c->dtype == MPC_E4M3)) ? 32 : 16;  // tiles_at_once
   // Fewer than 2^31 units (and half of that for the sums of their parts), by longer tiles where a table could hold more.
   while ((double)d->b * c->hk * pl->qt * (double)(d->max_pages * c->page_size / pl->tile + 1 + kItemCost) >= (double)(1 << 30)) {
     if (pl->tile >= (1 << 30)) return fail(MPC_ERR_UNSUPPORTED, "mpc_sdpa_paged: too many sequences and heads");
@@ -895,13 +908,14 @@ static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_d
   }
   // As many CTAs as are resident, fewer where even the longest lengths give fewer tiles than warps.
   const long long per = (d->max_pages * c->page_size + kWarps * pl->tile - 1) / (kWarps * pl->tile);
-  const long long sms = (long long)dev->prop.multiProcessorCount * (!tc ? 3 : pl->dp == 256 || pl->gt == 16 ? 2 : pl->dp == 64 ? D64_MINB : c->dtype == MPC_E4M3 ? E4_MINB : 3);
+  const long long sms = (long long)dev->prop.multiProcessorCount * (tc ? blocks_per_sm(c->dtype == MPC_E4M3, pl->dp, pl->gt) : 3);
   const long long heads = c->hk * pl->qt;
   long long ctas = sms;
   if (d->b > 0 && per > 0 && per <= sms / heads / d->b) ctas = per * heads * d->b;
   pl->ctas = (int)(ctas < 1 ? 1 : ctas);
-  pl->owners_bytes = (size_t)pl->ctas * kWarps * sizeof(int4);
-  pl->ws_bytes = pl->owners_bytes + (size_t)pl->ctas * kWarps * 2 * pl->gt * slot_floats((int)c->dv) * sizeof(float);
+  // The counters' room depends on the device alone, so that calls of any shape may follow one another in a workspace.
+  pl->counters_bytes = (size_t)dev->prop.multiProcessorCount * kMaxCtas * kWarps * sizeof(int);
+  pl->ws_bytes = pl->counters_bytes + (size_t)pl->ctas * kWarps * 2 * pl->gt * slot_floats((int)c->dv) * sizeof(float);
   return MPC_OK;
 }
 
@@ -955,10 +969,12 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
     return fail(MPC_ERR_INVALID, "mpc_sdpa_paged: null pointer");
   cudaStream_t st = stream_of(dev, s);
   Scratch own;
+  int *counters = dev->d_counters;  // the device stream's, whose calls follow one another
   if (workspace) {
     if (workspace_bytes < pl.ws_bytes || ((uintptr_t)workspace & 15))
       return fail(MPC_ERR_INVALID, "mpc_sdpa_paged: a workspace of %zu bytes at %p (%zu, 16-byte aligned, needed)",
                   workspace_bytes, workspace, pl.ws_bytes);
+    counters = static_cast<int *>(workspace);
   } else {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     MPC_CUDA(dev, cudaStreamIsCapturing(st, &cs));
@@ -966,15 +982,21 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
       return fail(MPC_ERR_INVALID, "mpc_sdpa_paged: a captured call needs a workspace of its own");
     if ((rc = own.get(dev, st, pl.ws_bytes))) return rc;
     workspace = own.ptr;
+    if (st != dev->stream || pl.counters_bytes > kCounterBytes) {
+      counters = static_cast<int *>(workspace);
+      MPC_CUDA(dev, cudaMemsetAsync(counters, 0, pl.counters_bytes, st));
+    }
   }
   Params p{};
   p.q = Q, p.kp = k_pages, p.vp = v_pages, p.ks = k_scale, p.vs = v_scale, p.table = table, p.lengths = lengths;
-  p.out = O, p.lse = LSE, p.err = dev->d_err, p.tile = pl.tile, p.owners = static_cast<int4 *>(workspace);
-  p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + pl.owners_bytes);
+  p.out = O, p.lse = LSE, p.err = dev->d_err, p.tile = pl.tile, p.counters = counters;
+  p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + pl.counters_bytes);
   for (int i = 0; i < 2; ++i) p.qs[i] = desc->q_stride[i], p.os[i] = desc->o_stride[i];
   p.max_pages = desc->max_pages, p.cap = desc->max_pages * cache->page_size;
   p.B = (int)desc->b, p.H = (int)desc->h, p.hk = (int)cache->hk, p.group = p.H / p.hk, p.gt = pl.gt, p.qt = pl.qt;
   p.d = (int)cache->d, p.dv = (int)cache->dv, p.page_size = (int)cache->page_size, p.n_pages = (int)cache->n_pages;
+  const size_t qb = dtype_size(desc->dtype);
+  p.q_vec = (((uintptr_t)Q | desc->q_stride[0] * qb | desc->q_stride[1] * qb) & 15) == 0;
   // With 2^(l-1) < page_size <= 2^l and page_mul = ceil(2^(31+l) / page_size) (below 2^32), page_mul * page_size exceeds
   // 2^(31+l) by less than 2^l, so the quotient is exact for keys below 2^31.
   int l = 0;
@@ -992,16 +1014,7 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
   else if (dm <= 128) vec ? launch_simt<2, true>(p, pl.ctas, st) : launch_simt<2, false>(p, pl.ctas, st);
   else vec ? launch_simt<4, true>(p, pl.ctas, st) : launch_simt<4, false>(p, pl.ctas, st);
   dev->launches++;
-  if ((rc = check_launch(dev, "mpc_sdpa_paged"))) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(pl.ctas, p.group < pl.gt ? p.group : pl.gt), cfg.blockDim = dim3(kThreads), cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  MPC_CUDA(dev, cudaLaunchKernelEx(&cfg, join_kernel, p));
-  dev->launches++;
-  return MPC_OK;
+  return check_launch(dev, "mpc_sdpa_paged");
 }
 
 }  // extern "C"

@@ -212,6 +212,7 @@ def test_workspace_of_the_caller_on_another_stream(be):
     need = C.c_size_t()
     F.call("mpc_sdpa_paged_workspace", dev.handle, c.args[0], C.byref(d), C.byref(need))
     ws, o = dev.alloc(need.value), dev.alloc(8 * 128 * 2)
+    dev.memset(ws.ptr, 0, ws.nbytes)
     dev.stream_sync()
     s = dev.new_stream()
 
@@ -219,8 +220,10 @@ def test_workspace_of_the_caller_on_another_stream(be):
         F.call("mpc_sdpa_paged", dev.handle, *c.args, C.byref(d), C.c_void_p(q.ptr), C.c_void_p(t.ptr), C.c_void_p(n.ptr),
                C.c_void_p(o.ptr), None, C.c_void_p(ws_ptr), nbytes, C.c_void_p(s))
 
-    call(ws.ptr, need.value)
-    assert np.array_equal(dev.download(o.ptr, o.nbytes, np.float16, (8 * 128,), stream=s), want)
+    for args in ((ws.ptr, need.value), (ws.ptr, need.value), (None, 0)):  # the workspace is ready for the next call
+        dev.memset(o.ptr, 255, o.nbytes, stream=s)
+        call(*args)
+        assert np.array_equal(dev.download(o.ptr, o.nbytes, np.float16, (8 * 128,), stream=s), want)
     for args in ((ws.ptr, need.value - 1), (ws.ptr + 8, need.value)):
         with pytest.raises(F.MpcError, match="workspace"):
             call(*args)
