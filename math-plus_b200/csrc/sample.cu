@@ -2,23 +2,38 @@
 // uniform number. It stands beside softmax, sort and argmax of the op set; the reference has no
 // sampler.
 //
-// All three filters keep a prefix of the tokens ranked by (logit descending, index ascending), so the
-// kept set is "every token above a threshold logit, and the first r tokens equal to it". Logits map to
-// 32-bit keys of the same order, and the threshold is found by radix selection: histograms of counts
-// and weights over 8 key bits at a time, from the top. No sort.
+// All three filters keep a prefix of the tokens ranked by (logit descending, index ascending), so the kept
+// set is "every token above a threshold logit, and the first r tokens equal to it", and no row is sorted:
+//   1. the largest logit;
+//   2. a histogram of counts over 4096 bins of T / 128 below it finds the bin where the ranks reach top_k, or
+//      estimates the one where the weights reach top_p of their total;
+//   3. the tokens of that bin and the bins above it (at most 2048; else the bin alone) are gathered and sorted,
+//      and the border is found among them exactly, with the exact weight of what lies above. A bin of more
+//      than 2048 tokens is cut again, by the bits of its logits; an estimate that was off moves on.
+//   4. Where the gathered tokens are the whole kept set (any usual top_k, a narrow top_p) the draw is among them.
+//      Else every warp sums the kept weights of its stretch of the row, and the one that the draw falls into
+//      walks its stretch.
+// Rows are read again by each step, from L1 or L2; HBM is read once.
 //
-// Weights w = exp((l - max) / T) in f64 are held as integers of 2^-shift (shift = 62 - log2 of the row's
-// length), so that sums are exact whatever their order: the same row always gives the same token, and
-// the borders of top-p and of the drawn interval move by less than 1e-12 of the total.
+// Weights w = exp((l - max) / T) in f64 are held as integers of 2^-shift (shift = 62 - log2 of the row's length, at
+// most 51), so that sums are exact whatever their order: the same row always gives the same token, and
+// the borders of top-p and of the drawn interval move by less than 1e-11 of the total.
 //
-// One CTA of 1024 threads per row; the row is read again by each pass, from L2.
+// A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy: a few rows are bound by latency, many by the
+// f64 exponentials of the rows without top_k (about 12 double operations a token) and by the passes over L2.
+#include <cooperative_groups.h>
+
 #include "kv_cache.cuh"
 #include "mpc_internal.h"
+
+namespace cg = cooperative_groups;
 
 namespace mpc {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 4096, kPer = kBins / kThreads, kList = 2048;
+constexpr float kBinsPerNat = 128.0f;
 
 struct SampleParams {
   const void *logits;
@@ -27,7 +42,7 @@ struct SampleParams {
   int32_t *token, *kept;
   float *prob;
   long long stride;
-  int vocab, dt, d_top_k, shift;
+  int vocab, d_top_k, shift;
   float d_temperature, d_top_p, d_min_p;
 };
 
@@ -36,216 +51,657 @@ __device__ __forceinline__ uint32_t key_of(float f) {
   const uint32_t b = __float_as_uint(f == 0.0f ? 0.0f : f);  // -0 ties with 0
   return !(f > -INFINITY) ? 0u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
 
-struct Row {
-  const void *x;
-  int dt;
-  float top;     // the largest logit
-  double inv_t;
-  int shift;
-  __device__ float logit(int i) const { return load_f32(x, dt, i); }
-  __device__ double weight(float f) const {
-    if (f == top) return 1.0;
-    const double d = ((double)f - (double)top) * inv_t;
-    return f > -INFINITY && d > -800.0 ? exp(d) : 0.0;
+typedef unsigned long long u64;
+
+struct Sums {  // one warp's stretch: kept weight and tokens above the threshold, tokens equal to it
+  u64 w;
+  unsigned n, ties;
+};
+struct Verdict {  // what the gathered tokens say
+  u64 total;
+  uint32_t key;
+  unsigned ties;
+  int again;
+};
+struct Shared {
+  double table[32];  // 2^(i / 32)
+  unsigned hist[kBins];  // later the merged list
+  unsigned cum[kBins];   // tokens in bins 0..b, of the whole row
+  u64 list[kList];
+  u64 best, scratch[kWarps], s_above, s_in, total;
+  Sums sums[kWarps], all[kWarps * kMaxCluster];
+  float fscratch[kWarps];
+  unsigned n_list, key_min, key_max;
+  int b0, b1;
+  Verdict verdict;
+};
+
+// Vectors of 16 bytes, aligned, over one row: vector v holds elements v * VE - mis ..+VE-1.
+template <int DT>
+struct Reader {
+  static constexpr int VE = DT == MPC_F32 ? 4 : 8;
+  using T = typename std::conditional<DT == MPC_F32, float, uint16_t>::type;
+  const T *x;
+  int V, mis, vectors;
+  __device__ void set(const void *base, long long at, int n) {
+    x = static_cast<const T *>(base) + at;
+    V = n;
+    mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+    vectors = (V + mis + VE - 1) / VE;
   }
-  __device__ unsigned long long whole(double w) const { return (unsigned long long)__double2ll_rn(ldexp(w, shift)); }
+  __device__ float one(int i) const {
+    if constexpr (DT == MPC_F32) return __ldg(x + i);
+    else if constexpr (DT == MPC_BF16) return __uint_as_float((uint32_t)__ldg(x + i) << 16);
+    else return __half2float(__ushort_as_half(__ldg(x + i)));
+  }
+  __device__ int index(int v) const { return v * VE - mis; }
+  __device__ void load(int v, float (&f)[VE]) const {
+    const int i0 = index(v);
+    if (i0 >= 0 && i0 + VE <= V) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4 *>(x + i0));
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (DT == MPC_F32) {
+          f[k] = __uint_as_float(w[k]);
+        } else {
+          const float2 p = DT == MPC_BF16 ? bf16x2_to_f32(w[k]) : f16x2_to_f32(w[k]);
+          f[2 * k] = p.x, f[2 * k + 1] = p.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) f[k] = i0 + k >= 0 && i0 + k < V ? one(i0 + k) : -INFINITY;
+    }
+  }
+  // fn(logit, index) over vectors v0 + lane, + 32, ..; elements outside the row come as -inf.
+  template <typename Fn>
+  __device__ __forceinline__ void each(int v0, int v1, Fn fn) const {
+    constexpr int U = 16 / VE;  // 64 bytes (f32) or 32 in flight
+    for (int v = v0 + (threadIdx.x & 31); v < v1; v += 32 * U) {
+      float f[U][VE];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v + 32 * u < v1) load(v + 32 * u, f[u]);
+        else
+#pragma unroll
+          for (int k = 0; k < VE; ++k) f[u][k] = -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < VE; ++k) fn(f[u][k], index(v + 32 * u) + k);
+    }
+  }
+};
+
+// w = 2^(y), y = (l - top) log2(e) / T, as 2^n * 2^(i / 32) * 2^r with |r| <= 1/64: the second from a table, the
+// last by its series to r^5 (the next term is below 3e-15).
+struct Weights {
+  double c, unit;  // log2(e) / T; 2^-shift
+  float top;
+  int shift;
+  const double *table;
+  __device__ __forceinline__ void parts(float f, double &s, double &p) const {
+    constexpr double L = 0.69314718055994530942;
+    double y = f == top ? 0.0 : ((double)f - (double)top) * c;
+    y = fmax(y, -1000.0);  // also for NaN: logits below an infinite one
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
+    const double t = fma(y, 32.0, magic);
+    const int k = __double2loint(t);
+    const double r = fma(t - magic, -1.0 / 32, y);
+    p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
+    p = fma(p, r, L * L * L / 6);
+    p = fma(p, r, L * L / 2);
+    p = fma(p, r, L);
+    p = fma(p, r, 1.0);
+    const double e = table[k & 31];
+    s = __hiloint2double(__double2hiint(e) + ((k >> 5) + shift) * (1 << 20), __double2loint(e));
+  }
+  __device__ __forceinline__ double weight(float f) const {
+    double s, p;
+    parts(f, s, p);
+    return s * p * unit;
+  }
+  // The nearest whole number of units: below 2^52, so it appears in the low bits next to 2^52.
+  __device__ __forceinline__ u64 whole(float f) const {
+    double s, p;
+    parts(f, s, p);
+    return (u64)__double_as_longlong(fma(s, p, 4503599627370496.0)) - 0x4330000000000000ull;
+  }
 };
 
 template <typename T>
-__device__ T block_sum(T v, T *sm) {
-#pragma unroll
-  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T all = 0;
-  for (int i = 0; i < kThreads / 32; ++i) all += sm[i];
-  return all;
-}
-
-// Exclusive prefix sum over the threads.
-template <typename T>
-__device__ T block_before(T v, T *sm) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  T incl = v;
+__device__ __forceinline__ T warp_incl(T v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const T u = __shfl_up_sync(0xffffffffu, incl, m);
-    if (lane >= m) incl += u;
+    const T o = __shfl_up_sync(0xffffffffu, v, m);
+    if (lane >= m) v += o;
   }
+  return v;
+}
+// Inclusive prefix over the block's threads; *all: the sum.
+template <typename T>
+__device__ __forceinline__ T block_incl(T v, T *sm, T *all) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  v = warp_incl(v);
   __syncthreads();
-  if (lane == 31) sm[w] = incl;
+  if (lane == 31) sm[w] = v;
   __syncthreads();
-  T before = 0;
-  for (int i = 0; i < w; ++i) before += sm[i];
-  return before + incl - v;
+  T before = 0, sum = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < w) before += sm[i];
+    sum += sm[i];
+  }
+  *all = sum;
+  return v + before;
 }
 
-struct Shared {
-  unsigned long long w[256], sum[32];
-  unsigned n[256], cnt[32];
-  unsigned long long w_above;
-  unsigned n_above, prefix, n_at;
+// Sorts n2 (a power of two) numbers in shared memory, descending or ascending.
+__device__ void sort(u64 *a, int n2, bool descending) {
+  for (int k = 2; k <= n2; k <<= 1)
+    for (int j = k >> 1; j; j >>= 1) {
+      __syncthreads();
+      for (int q = threadIdx.x; q < n2 / 2; q += kThreads) {
+        const int i = (q & ~(j - 1)) << 1 | (q & (j - 1)), l = i + j;
+        const u64 x = a[i], y = a[l];
+        if ((x < y) == (((i & k) == 0) == descending)) a[i] = y, a[l] = x;
+      }
+    }
+  __syncthreads();
+}
+
+// The histogram's bins: by value below the largest logit, or by the keys of an interval.
+struct Bins {
+  float top, scale;  // bins of T / 128 below top
+  uint32_t lo, hi;   // keys of the interval (lo 0: all, by value)
+  int shift;
+  __device__ __forceinline__ int of(float f, uint32_t key) const {
+    if (lo) return (int)((hi - key) >> shift);
+    const float x = f == top ? 0.0f : (top - f) * scale;
+    return x < kBins - 1 ? (int)x : x >= kBins - 1 ? kBins - 1 : 0;  // NaN (a scale of inf or 0): 0
+  }
+  // The weight of a bin's middle, for estimates.
+  __device__ __forceinline__ float middle(int b, float per_nat) const {
+    if (!lo) return __expf(-((float)b + 0.5f) / kBinsPerNat);
+    const uint32_t k = hi - min(hi - lo, ((uint32_t)b << shift) + ((1u << shift) >> 1));
+    const float x = (top - logit_of(k)) * per_nat;
+    return x > 0.0f ? __expf(-x) : 1.0f;
+  }
 };
 
-// The key at which the ranked tokens' running count (or, with BY_WEIGHT, weight) reaches `want`:
-// sm.prefix, with sm.n_above tokens of weight sm.w_above above it and sm.n_at equal to it.
-template <bool BY_WEIGHT>
-__device__ void select(const Row &r, int vocab, unsigned long long want, Shared &sm) {
-  if (threadIdx.x == 0) sm.prefix = 0, sm.n_above = 0, sm.w_above = 0;
-  for (int bits = 24; bits >= 0; bits -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kThreads) sm.n[i] = 0, sm.w[i] = 0;
-    __syncthreads();
-    const uint32_t prefix = sm.prefix;
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-      const float f = r.logit(i);
-      const uint32_t k = key_of(f);
-      if (k == 0 || (bits < 24 && (k >> (bits + 8)) != prefix)) continue;
-      atomicAdd(&sm.n[(k >> bits) & 255], 1u);
-      atomicAdd(&sm.w[(k >> bits) & 255], r.whole(r.weight(f)));
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      unsigned n = sm.n_above;
-      unsigned long long w = sm.w_above;
-      int last = 0;
-      for (int i = 255; i >= 0; --i) {
-        if (!sm.n[i]) continue;
-        last = i;
-        if (BY_WEIGHT ? w + sm.w[i] >= want : n + sm.n[i] >= want) break;
-        n += sm.n[i], w += sm.w[i];
-      }
-      if (BY_WEIGHT ? w + sm.w[last] < want : n + sm.n[last] < want) n -= sm.n[last], w -= sm.w[last];  // all of them
-      sm.n_above = n, sm.w_above = w, sm.prefix = prefix << 8 | last, sm.n_at = sm.n[last];
-    }
-    __syncthreads();
-  }
-}
-
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
-  __shared__ Shared sm;
-  const int row = blockIdx.x, V = p.vocab;
-  Row r;
-  r.dt = p.dt;
-  r.x = static_cast<const uint8_t *>(p.logits) + (long long)row * p.stride * (p.dt == MPC_F32 ? 4 : 2);
-  r.shift = p.shift;
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Shared &sm = *reinterpret_cast<Shared *>(raw);
+  const auto cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int row = blockIdx.x / C, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Reader<DT> rd;
+  rd.set(p.logits, row * p.stride, p.vocab);
+  const int per_cta = (rd.vectors + C - 1) / C, per_warp = (per_cta + kWarps - 1) / kWarps;
+  const int c1 = min(rd.vectors, (rank + 1) * per_cta);
+  const int v0 = min(c1, rank * per_cta + warp * per_warp), v1 = min(c1, v0 + per_warp);
   const float t = p.temperature ? p.temperature[row] : p.d_temperature;
   const float top_p = p.top_p ? p.top_p[row] : p.d_top_p;
   const float min_p = p.min_p ? p.min_p[row] : p.d_min_p;
   const int top_k = p.top_k ? p.top_k[row] : p.d_top_k;
+  if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
 
-  // The largest logit and its lowest index, as the pair (key, ~index).
-  unsigned long long best = 0;
-  for (int i = threadIdx.x; i < V; i += kThreads) {
-    const unsigned long long c = (unsigned long long)key_of(r.logit(i)) << 32 | (0xffffffffu - (unsigned)i);
-    best = c > best ? c : best;
-  }
+  // 1. The largest logit and its lowest index, as the pair (key, ~index).
+  u64 best = 0;
+  {
+    float f_best = -INFINITY;
+    int at = -1;
+    rd.each(v0, v1, [&](float f, int i) {
+      if (f > f_best) f_best = f, at = i;
+    });
+    best = (u64)key_of(f_best) << 32 | (0xffffffffu - (unsigned)at);
 #pragma unroll
-  for (int m = 16; m; m >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, m);
-    best = o > best ? o : best;
+    for (int m = 16; m; m >>= 1) {
+      const u64 o = __shfl_xor_sync(0xffffffffu, best, m);
+      best = o > best ? o : best;
+    }
+    if (lane == 0) sm.scratch[warp] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) best = sm.scratch[i] > best ? sm.scratch[i] : best;
+    if (threadIdx.x == 0) sm.best = best;
+    cl.sync();
+    for (int i = 0; i < C; ++i) {
+      const u64 o = *cl.map_shared_rank(&sm.best, i);
+      best = o > best ? o : best;
+    }
   }
-  if ((threadIdx.x & 31) == 0) sm.sum[threadIdx.x >> 5] = best;
-  __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) best = sm.sum[i] > best ? sm.sum[i] : best;
   const uint32_t top_key = (uint32_t)(best >> 32);
-  const int top_at = (int)(0xffffffffu - (uint32_t)best);
   if (top_key == 0 || !(t > 0.0f)) {
-    if (threadIdx.x == 0) {
-      p.token[row] = top_key ? top_at : -1;
+    if (rank == 0 && threadIdx.x == 0) {
+      p.token[row] = top_key ? (int)(0xffffffffu - (uint32_t)best) : -1;
       if (p.prob) p.prob[row] = top_key ? 1.0f : 0.0f;
       if (p.kept) p.kept[row] = top_key ? 1 : 0;
     }
+    cl.sync();  // nobody reads a CTA that has gone
     return;
   }
-  r.top = r.logit(top_at);
-  r.inv_t = 1.0 / (double)t;
-  __syncthreads();
+  Weights wt;
+  wt.top = logit_of(top_key);
+  wt.c = 1.4426950408889634074 / (double)t;
+  wt.shift = p.shift;
+  wt.unit = ldexp(1.0, -p.shift);
+  wt.table = sm.table;
+  const float u = fminf(fmaxf(p.u[row], 0.0f), 1.0f);
+  auto draw_of = [&](u64 total) {
+    const u64 d = (u64)__double2ll_rd((double)u * (double)total);
+    return d < total ? d : total - 1;
+  };
+  auto passes = [&](uint32_t key, double w) { return key == top_key || !(w < (double)min_p); };
 
-  // Kept: keys above `key`, and the first `ties` tokens of that key.
+  // 2., 3. The threshold: keys above `key` are kept, and the first `ties` tokens of that key.
   uint32_t key = 0;
   unsigned ties = 0;
-  unsigned long long total = 0;
-  const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.0f;
-  if (by_k) {
-    select<false>(r, V, (unsigned long long)top_k, sm);
-    key = sm.prefix;
-    ties = min(sm.n_at, (unsigned)top_k - sm.n_above);
-    const uint32_t b = (key & 0x80000000u) ? (key & 0x7fffffffu) : ~key;
-    total = sm.w_above + ties * r.whole(r.weight(__uint_as_float(b)));
-    __syncthreads();
-  } else if (by_p) {
-    unsigned long long w = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads) w += r.whole(r.weight(r.logit(i)));
-    total = block_sum(w, sm.sum);
-    __syncthreads();
-  }
-  if (by_p) {
-    // The ranks before which less than top_p * total lies: those whose preceding weight is < want.
-    const double lim = top_p > 0.0f ? (double)top_p * (double)total : 0.0;
-    unsigned long long want = (unsigned long long)__double2ll_ru(lim);
-    if (want < 1) want = 1;
-    if (want > total) want = total;
-    select<true>(r, V, want, sm);
-    const uint32_t at = sm.prefix;
-    const uint32_t b = (at & 0x80000000u) ? (at & 0x7fffffffu) : ~at;
-    const unsigned long long w = r.whole(r.weight(__uint_as_float(b)));
-    unsigned n = sm.n_at;
-    if (w > 0) {
-      const unsigned long long need = (want - sm.w_above + w - 1) / w;
-      if (need < n) n = (unsigned)need;
-    }
-    if (at > key || (at == key && n < ties)) key = at, ties = n;
-    __syncthreads();
-  }
-
-  // Thread i's tokens are [i c, (i + 1) c): the kept weight and number before them give the place of the draw.
-  const int c = (V + kThreads - 1) / kThreads;
-  const int i0 = min(V, (int)threadIdx.x * c), i1 = min(V, i0 + c);
-  unsigned at_key = 0;
-  if (key)
-    for (int i = i0; i < i1; ++i) at_key += key_of(r.logit(i)) == key;
-  unsigned tie = block_before(at_key, sm.cnt);
-  const unsigned tie0 = tie;
-  unsigned long long mine = 0;
-  unsigned count = 0;
-  auto keeps = [&](float f, double w) {
-    const uint32_t k = key_of(f);
-    if (k == 0 || k < key) return false;
-    if (k == key && tie++ >= ties) return false;
-    return k == top_key || !(w < (double)min_p);
-  };
-  for (int i = i0; i < i1; ++i) {
-    const float f = r.logit(i);
-    const double w = r.weight(f);
-    if (keeps(f, w)) mine += r.whole(w), ++count;
-  }
-  __syncthreads();
-  count = block_sum(count, sm.cnt);
-  __syncthreads();
-  total = block_sum(mine, sm.sum);
-  __syncthreads();
-  const unsigned long long before = block_before(mine, sm.sum);
-  const float u = fminf(fmaxf(p.u[row], 0.0f), 1.0f);
-  unsigned long long want = (unsigned long long)__double2ll_rd((double)u * (double)total);
-  if (want >= total) want = total - 1;
-  if (before <= want && want < before + mine) {
-    tie = tie0;
-    unsigned long long sum = before;
-    for (int i = i0; i < i1; ++i) {
-      const float f = r.logit(i);
-      const double w = r.weight(f);
-      if (!keeps(f, w)) continue;
-      sum += r.whole(w);
-      if (sum > want) {
-        p.token[row] = i;
-        if (p.prob) p.prob[row] = (float)(w / ldexp((double)total, -r.shift));
+  bool by_k = top_k > 0 && top_k < p.vocab;
+  const bool by_p = top_p < 1.0f;
+  if (by_k || by_p) {
+    Bins bins;
+    bins.top = wt.top, bins.scale = kBinsPerNat / t, bins.lo = bins.hi = 0, bins.shift = 0;
+    bool counting = by_k;
+    unsigned n_above = 0;           // tokens above the interval
+    u64 base = 0, span = 0;         // weight above it, in it (by weight)
+    u64 total = 0, want = 0;        // by weight: ranks before which less than `want` lies are kept
+    bool known = false;             // total is
+    auto want_of = [&](u64 sum) {
+      const double lim = top_p > 0.0f ? (double)top_p * (double)sum : 0.0;
+      const u64 w = (u64)__double2ll_ru(lim);
+      return w < 1 ? 1 : w > sum ? sum : w;
+    };
+    for (bool found = false; !found;) {
+      // The histogram of the interval.
+      for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
+      __syncthreads();
+      u64 w = 0;
+      unsigned deep = 0;
+      const bool weigh = !counting && !known;
+      rd.each(v0, v1, [&](float f, int) {
+        const uint32_t k = key_of(f);
+        if (k == 0 || (bins.lo && (k < bins.lo || k > bins.hi))) return;
+        const int b = bins.of(f, k);
+        if (b == kBins - 1) ++deep;
+        else atomicAdd(&sm.hist[b], 1u);
+        if (weigh) w += wt.whole(f);
+      });
+      u64 sum;
+      block_incl(w, sm.scratch, &sum);
+      if (threadIdx.x == 0) sm.total = sum;
+      for (int m = 16; m; m >>= 1) deep += __shfl_xor_sync(0xffffffffu, deep, m);
+      if (lane == 0 && deep) atomicAdd(&sm.hist[kBins - 1], deep);
+      cl.sync();
+      unsigned cnt[kPer] = {};
+      for (int i = 0; i < C; ++i) {
+        const uint4 *h = reinterpret_cast<const uint4 *>(cl.map_shared_rank(sm.hist, i) + threadIdx.x * kPer);
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j) {
+          const uint4 x = h[j];
+          cnt[4 * j] += x.x, cnt[4 * j + 1] += x.y, cnt[4 * j + 2] += x.z, cnt[4 * j + 3] += x.w;
+        }
+        if (weigh) total += *cl.map_shared_rank(&sm.total, i);
+      }
+      if (weigh) known = true, want = want_of(total), span = total;
+      unsigned mine = 0, tokens;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) mine += cnt[j];
+      unsigned before = block_incl(mine, reinterpret_cast<unsigned *>(sm.scratch), &tokens) - mine;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const unsigned incl = before + cnt[j];
+        sm.cum[threadIdx.x * kPer + j] = incl;
+        if (counting && n_above + before < (unsigned)top_k && n_above + incl >= (unsigned)top_k) sm.b1 = threadIdx.x * kPer + j;
+        before = incl;
+      }
+      __syncthreads();
+      if (counting && n_above + tokens < (unsigned)top_k) {  // fewer tokens than top_k
+        by_k = counting = false;
+        if (!by_p) break;
+        cl.sync();
+        continue;
+      }
+      auto pop = [&](int a, int b) { return sm.cum[b] - (a ? sm.cum[a - 1] : 0u); };
+      // The bin where the estimated weights reach `goal`, within [lo, hi], into sm.b1.
+      auto by_weight = [&](float goal, int lo, int hi) {
+        float e[kPer], part = 0.0f, all;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int b = threadIdx.x * kPer + j;
+          e[j] = (float)pop(b, b) * bins.middle(b, 1.0f / t);
+          part += e[j];
+        }
+        float upto = block_incl(part, sm.fscratch, &all) - part;
+        if (threadIdx.x == 0) sm.b1 = hi;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          upto += e[j];
+          if (upto >= goal) atomicMin(&sm.b1, threadIdx.x * kPer + j);
+        }
+        __syncthreads();
+        const int b = max(sm.b1, lo);
+        __syncthreads();
+        return b;
+      };
+      auto estimate = [&](int upto) {  // of the weights of bins 0..upto
+        float part = 0.0f, all;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int b = threadIdx.x * kPer + j;
+          if (b <= upto) part += (float)pop(b, b) * bins.middle(b, 1.0f / t);
+        }
+        block_incl(part, sm.fscratch, &all);
+        return all;
+      };
+      int bx;
+      if (counting) bx = sm.b1;
+      else bx = by_weight(span ? estimate(kBins - 1) * (float)((double)(want - base) / (double)span) : (float)((double)(want - base) * wt.unit), 0, kBins - 1);
+      for (;;) {
+        // The window [b0, b1]: all down to the border where the list holds that, else the bins next to it.
+        int b1 = counting ? bx : min(bx + 1, kBins - 1);
+        int b0 = pop(0, b1) <= kList ? 0 : counting ? bx : max(bx - 1, 0);
+        if (pop(b0, b1) > kList) b0 = b1 = bx;
+        const bool gather = pop(b0, b1) <= kList;
+        const bool need = !counting || by_p;
+        __syncthreads();
+        if (threadIdx.x == 0) sm.n_list = 0, sm.key_min = 0xffffffffu, sm.key_max = 0;
+        __syncthreads();
+        u64 above = 0, in = 0;
+        rd.each(v0, v1, [&](float f, int i) {
+          const uint32_t k = key_of(f);
+          if (k == 0 || (bins.lo && k < bins.lo)) return;
+          const int b = bins.lo && k > bins.hi ? -1 : bins.of(f, k);
+          if (b < b0) {
+            if (need) above += wt.whole(f);
+          } else if (b <= b1) {
+            if (!counting) in += wt.whole(f);
+            if (gather) sm.list[atomicAdd(&sm.n_list, 1u)] = (u64)k << 32 | (0xffffffffu - (unsigned)i);
+            else atomicMin(&sm.key_min, k), atomicMax(&sm.key_max, k);
+          }
+        });
+        block_incl(above, sm.scratch, &sum);
+        if (threadIdx.x == 0) sm.s_above = sum;
+        block_incl(in, sm.scratch, &sum);
+        if (threadIdx.x == 0) sm.s_in = sum;
+        cl.sync();
+        above = in = 0;
+        uint32_t kmin = 0xffffffffu, kmax = 0;
+        for (int i = 0; i < C; ++i) {
+          above += *cl.map_shared_rank(&sm.s_above, i);
+          in += *cl.map_shared_rank(&sm.s_in, i);
+          kmin = min(kmin, *cl.map_shared_rank(&sm.key_min, i));
+          kmax = max(kmax, *cl.map_shared_rank(&sm.key_max, i));
+        }
+        if (!counting && want <= above) {  // the border lies further up
+          const float e = estimate(b0 - 1);
+          bx = min(b0 - 1, by_weight((float)(e * ((double)(want - base) / (double)(above - base))), 0, b0 - 1));
+          cl.sync();
+          continue;
+        }
+        if (!counting && want > above + in) {  // further down
+          const float e = estimate(b1);
+          bx = by_weight((float)(e * ((double)(want - base) / (double)(above + in - base))), b1 + 1, kBins - 1);
+          cl.sync();
+          continue;
+        }
+        const unsigned over = n_above + (b0 ? sm.cum[b0 - 1] : 0u);  // tokens above the window
+        if (!gather && kmin < kmax) {  // cut the window again by its keys
+          bins.lo = kmin, bins.hi = kmax, bins.shift = 0;
+          while (((kmax - kmin) >> bins.shift) >= kBins) ++bins.shift;
+          n_above = over, base = above, span = counting ? 0 : in;
+          cl.sync();
+          break;
+        }
+        if (!gather) {  // more equal logits than the list holds
+          const u64 each = wt.whole(logit_of(kmin));
+          key = kmin;
+          found = true;
+          if (counting) {
+            ties = (unsigned)top_k - over;
+            if (by_p) {
+              total = above + ties * each, want = want_of(total);
+              if (want <= above) found = false;
+            }
+          } else {
+            ties = pop(b0, b1);
+          }
+          if (found && by_p && each) ties = (unsigned)min((u64)ties, (want - above + each - 1) / each);
+          if (!found) {  // top-p's border lies above top-k's: find it by weight, from the whole row
+            counting = false, known = true, base = span = 0, n_above = 0, bins.lo = 0;
+          }
+          cl.sync();
+          break;
+        }
+        // The first CTA sorts the gathered tokens and finds the border among them.
+        if (rank == 0) {
+          u64 *const all = reinterpret_cast<u64 *>(sm.hist);
+          int n = 0;
+          for (int i = 0; i < C; ++i) {
+            const int m = (int)*cl.map_shared_rank(&sm.n_list, i);
+            const u64 *from = cl.map_shared_rank(sm.list, i);
+            for (int j = threadIdx.x; j < m; j += kThreads) all[n + j] = from[j];
+            n += m;
+          }
+          int n2 = 32;
+          while (n2 < n) n2 <<= 1;
+          for (int j = n + threadIdx.x; j < n2; j += kThreads) all[j] = 0;
+          sort(all, n2, true);
+          const int lim = counting ? min(n, (int)((unsigned)top_k - over)) : n;
+          // Thread i weighs ranks 4i ..+3.
+          u64 q[kList / kThreads], part = 0;
+          const int r0 = threadIdx.x * (kList / kThreads);
+#pragma unroll
+          for (int j = 0; j < kList / kThreads; ++j) {
+            q[j] = r0 + j < lim && by_p ? wt.whole(logit_of((uint32_t)(all[r0 + j] >> 32))) : 0;
+            part += q[j];
+          }
+          u64 upto = block_incl(part, sm.scratch, &sum) - part;
+          u64 goal = want;
+          bool again = false;
+          if (counting && by_p) {
+            total = above + sum, goal = want_of(total);
+            again = goal <= above;
+          }
+          unsigned kept = 0;
+          upto += above;
+#pragma unroll
+          for (int j = 0; j < kList / kThreads; ++j) {
+            kept += r0 + j < lim && (!by_p || upto < goal);
+            upto += q[j];
+          }
+          unsigned n_kept;
+          block_incl(kept, reinterpret_cast<unsigned *>(sm.scratch), &n_kept);
+          if (over == 0) {
+            // 4. The kept set is among the gathered tokens: min-p, then the draw in the order of the indices.
+            kept = 0;
+            for (unsigned j = threadIdx.x; j < n_kept; j += kThreads) {
+              const uint32_t k = (uint32_t)(all[j] >> 32);
+              kept += passes(k, wt.weight(logit_of(k)));
+            }
+            block_incl(kept, reinterpret_cast<unsigned *>(sm.scratch), &n_kept);
+            n2 = 32;
+            while (n2 < (int)n_kept) n2 <<= 1;
+            for (int j = threadIdx.x; j < n2; j += kThreads) {
+              const u64 x = all[j];
+              all[j] = j < (int)n_kept ? (u64)(0xffffffffu - (uint32_t)x) << 32 | x >> 32 : ~0ull;
+            }
+            sort(all, n2, false);
+            part = 0;
+#pragma unroll
+            for (int j = 0; j < kList / kThreads; ++j) {
+              q[j] = r0 + j < (int)n_kept ? wt.whole(logit_of((uint32_t)all[r0 + j])) : 0;
+              part += q[j];
+            }
+            upto = block_incl(part, sm.scratch, &sum) - part;
+            const u64 d = draw_of(sum);
+#pragma unroll
+            for (int j = 0; j < kList / kThreads; ++j) {
+              if (upto <= d && d < upto + q[j]) {
+                const u64 x = all[r0 + j];
+                p.token[row] = (int32_t)(x >> 32);
+                if (p.prob) p.prob[row] = (float)(wt.weight(logit_of((uint32_t)x)) / ((double)sum * wt.unit));
+              }
+              upto += q[j];
+            }
+            if (threadIdx.x == 0 && p.kept) p.kept[row] = (int32_t)n_kept;
+          } else if (threadIdx.x == 0) {
+            Verdict v;
+            v.total = total, v.again = again, v.key = 0, v.ties = 0;
+            if (!again) {
+              v.key = (uint32_t)(all[n_kept - 1] >> 32);
+              for (int j = (int)n_kept - 1; j >= 0 && (uint32_t)(all[j] >> 32) == v.key; --j) ++v.ties;
+            }
+            sm.verdict = v;
+          }
+        }
+        cl.sync();
+        if (over == 0) return;  // the first CTA has drawn
+        const Verdict v = *cl.map_shared_rank(&sm.verdict, 0);
+        cl.sync();
+        if (v.again) {
+          counting = false, known = true, base = span = 0, n_above = 0, bins.lo = 0;
+          total = v.total, want = want_of(total);
+        } else {
+          key = v.key, ties = v.ties, found = true;
+        }
         break;
       }
     }
   }
-  if (threadIdx.x == 0 && p.kept) p.kept[row] = (int32_t)count;
+
+  // 4. Every warp's kept weight, and the one that the draw falls into.
+  float far = -INFINITY;  // below it w < min_p for sure
+  if (min_p > 0.0f) {
+    const float x = wt.top + t * logf(min_p) - (0.01f * t + 1e-6f * fabsf(wt.top));
+    if (x == x) far = fminf(x, wt.top);
+  }
+  {
+    Sums s{0, 0, 0};
+    rd.each(v0, v1, [&](float f, int) {
+      const uint32_t k = key_of(f);
+      if (k == 0 || k < key || f < far) return;
+      if (k == key) {
+        ++s.ties;
+        return;
+      }
+      double a, b;
+      wt.parts(f, a, b);
+      if (min_p > 0.0f && !passes(k, a * b * wt.unit)) return;
+      s.w += (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - 0x4330000000000000ull;
+      ++s.n;
+    });
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+      s.w += __shfl_xor_sync(0xffffffffu, s.w, m);
+      s.n += __shfl_xor_sync(0xffffffffu, s.n, m);
+      s.ties += __shfl_xor_sync(0xffffffffu, s.ties, m);
+    }
+    if (lane == 0) sm.sums[warp] = s;
+  }
+  cl.sync();
+  for (int i = threadIdx.x; i < C * kWarps; i += kThreads) sm.all[i] = cl.map_shared_rank(sm.sums, i / kWarps)[i % kWarps];
+  __syncthreads();
+  const u64 tie_w = key ? wt.whole(logit_of(key)) : 0;
+  if (key && !passes(key, wt.weight(logit_of(key)))) ties = 0;
+  // Each warp walks the stretches up to its own, lane by lane of 32.
+  u64 total = 0, before = 0, mine = 0;
+  unsigned kept = 0, tie_before = 0, tie_at = 0;
+  const int self = rank * kWarps + warp;
+  for (int i0 = 0; i0 < C * kWarps; i0 += 32) {
+    Sums s{0, 0, 0};
+    if (i0 + lane < C * kWarps) s = sm.all[i0 + lane];
+    const unsigned tie_incl = tie_at + warp_incl(s.ties), tie_excl = tie_incl - s.ties;
+    const unsigned take = min(ties, tie_incl) - min(ties, tie_excl);
+    const u64 w = s.w + take * tie_w, incl = total + warp_incl(w);
+    const unsigned n = warp_incl(s.n + take);
+    if (i0 <= self && self < i0 + 32) {
+      mine = __shfl_sync(0xffffffffu, w, self - i0);
+      before = __shfl_sync(0xffffffffu, incl, self - i0) - mine;
+      tie_before = __shfl_sync(0xffffffffu, tie_excl, self - i0);
+    }
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    kept += __shfl_sync(0xffffffffu, n, 31);
+    tie_at = __shfl_sync(0xffffffffu, tie_incl, 31);
+  }
+  if (rank == 0 && threadIdx.x == 0 && p.kept) p.kept[row] = (int32_t)kept;
+  const u64 d = draw_of(total);
+  if (before <= d && d < before + mine) {
+    constexpr int VE = Reader<DT>::VE;
+    u64 at = before;
+    unsigned tie = tie_before;
+    for (int v = v0; v < v1; v += 32) {
+      float f[VE];
+#pragma unroll
+      for (int k = 0; k < VE; ++k) f[k] = -INFINITY;
+      if (v + lane < v1) rd.load(v + lane, f);
+      unsigned eq = 0;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) eq += key && key_of(f[k]) == key;
+      const unsigned eq_incl = warp_incl(eq);
+      unsigned my_tie = tie + eq_incl - eq;
+      u64 q[VE], part = 0;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        const uint32_t kk = key_of(f[k]);
+        q[k] = 0;
+        if (kk == 0 || kk < key || f[k] < far) continue;
+        if (kk == key) {
+          if (my_tie++ < ties) q[k] = tie_w;
+        } else if (!(min_p > 0.0f) || passes(kk, wt.weight(f[k]))) {
+          q[k] = wt.whole(f[k]);
+        }
+        part += q[k];
+      }
+      const u64 incl = at + warp_incl(part);
+      u64 upto = incl - part;
+      if (upto <= d && d < incl) {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          if (upto <= d && d < upto + q[k]) {
+            p.token[row] = rd.index(v + lane) + k;
+            if (p.prob) p.prob[row] = (float)(wt.weight(f[k]) / ((double)total * wt.unit));
+          }
+          upto += q[k];
+        }
+      }
+      at = __shfl_sync(0xffffffffu, incl, 31);
+      if (at > d) break;
+      tie += __shfl_sync(0xffffffffu, eq_incl, 31);
+    }
+  }
+  cl.sync();
+}
+
+template <int DT>
+int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
+  static bool configured[64] = {};
+  const int ord = dev->ordinal & 63;
+  if (!configured[ord]) {
+    MPC_CUDA(dev, cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+    configured[ord] = true;
+  }
+  // CTAs per row: up to two for every SM, of at least 2048 tokens.
+  int c = 1;
+  while (c < kMaxCluster && (long long)rows * c < 2ll * dev->prop.multiProcessorCount && p.vocab >= 2 * c * 2048) c *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)rows * c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sizeof(Shared), cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)c, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  MPC_CUDA(dev, cudaLaunchKernelEx(&cfg, sample_kernel<DT>, p));
+  dev->launches++;
+  return MPC_OK;
 }
 
 }  // namespace
@@ -269,12 +725,14 @@ extern "C" int mpc_sample(mpc_device *dev, const mpc_sample_desc *d, const void 
   if (!logits || !u || !token) return fail(MPC_ERR_INVALID, "mpc_sample: null pointer");
   SampleParams p{};
   p.logits = logits, p.u = u, p.temperature = temperature, p.top_p = top_p, p.min_p = min_p, p.top_k = top_k;
-  p.token = token, p.kept = kept, p.prob = prob, p.stride = d->row_stride, p.vocab = (int)d->vocab, p.dt = d->dtype;
+  p.token = token, p.kept = kept, p.prob = prob, p.stride = d->row_stride, p.vocab = (int)d->vocab;
   p.d_top_k = d->top_k, p.d_temperature = d->temperature, p.d_top_p = d->top_p, p.d_min_p = d->min_p;
   int log2v = 0;
   while ((int64_t(1) << log2v) < d->vocab) ++log2v;
-  p.shift = 62 - log2v;  // V weights of at most 2^shift stay below 2^63
-  sample_kernel<<<(unsigned)d->rows, kThreads, 0, stream_of(dev, s)>>>(p);
-  dev->launches++;
-  return check_launch(dev, "mpc_sample");
+  p.shift = log2v < 11 ? 51 : 62 - log2v;  // V weights of at most 2^shift stay below 2^63, each below 2^52
+  cudaStream_t st = stream_of(dev, s);
+  const int rows = (int)d->rows;
+  if (d->dtype == MPC_F32) return launch_sample<MPC_F32>(dev, p, rows, st);
+  if (d->dtype == MPC_BF16) return launch_sample<MPC_BF16>(dev, p, rows, st);
+  return launch_sample<MPC_F16>(dev, p, rows, st);
 }
