@@ -72,7 +72,7 @@ struct Shared {
   unsigned hist[kBins];  // later the merged list
   unsigned cum[kBins];   // tokens in bins 0..b, of the whole row
   u64 list[kList];
-  u64 best, scratch[kWarps], s_above, s_in, total;
+  u64 scratch[kWarps], s_above, s_in, total;
   Sums sums[kWarps], all[kWarps * kMaxCluster];
   float fscratch[kWarps];
   unsigned n_list, key_min, key_max;
@@ -117,6 +117,35 @@ struct Reader {
 #pragma unroll
       for (int k = 0; k < VE; ++k) f[k] = i0 + k >= 0 && i0 + k < V ? one(i0 + k) : -INFINITY;
     }
+  }
+  // The largest of a thread's elements of vectors v0 + lane, + 32, ..; -inf where there is none.
+  __device__ __forceinline__ float largest(int v0, int v1) const {
+    float best = -INFINITY;
+    if constexpr (DT == MPC_F32) {
+      each(v0, v1, [&](float f, int) { best = fmaxf(best, f); });
+    } else {
+      // Pairs by the packed maximum of the type (a NaN gives the other number).
+      uint32_t m = DT == MPC_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+      for (int v = v0 + (threadIdx.x & 31); v < v1; v += 32) {
+        const int i0 = index(v);
+        if (i0 >= 0 && i0 + VE <= V) {
+          const uint4 r = __ldg(reinterpret_cast<const uint4 *>(x + i0));
+          m = max2(m, max2(max2(r.x, r.y), max2(r.z, r.w)));
+        } else {
+          for (int k = 0; k < VE; ++k)
+            if (i0 + k >= 0 && i0 + k < V) best = fmaxf(best, one(i0 + k));
+        }
+      }
+      const float2 p = DT == MPC_BF16 ? bf16x2_to_f32(m) : f16x2_to_f32(m);
+      best = fmaxf(best, fmaxf(p.x, p.y));
+    }
+    return best;
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == MPC_BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
   }
   // fn(logit, index) over vectors v0 + lane, + 32, ..; elements outside the row come as -inf.
   template <typename Fn>
@@ -217,22 +246,26 @@ __device__ void sort(u64 *a, int n2, bool descending) {
   __syncthreads();
 }
 
-// The histogram's bins: by value below the largest logit, or by the keys of an interval.
+// The histogram's bins: by value below the largest logit (the last bin is not used: what lies deeper is not
+// counted), or by the keys of an interval.
 struct Bins {
-  float top, scale;  // bins of T / 128 below top
-  uint32_t lo, hi;   // keys of the interval (lo 0: all, by value)
+  float top, scale;  // by value: bins of T / 128
+  uint32_t lo, hi;   // by key: the interval; lo 0: by value
   int shift;
-  __device__ __forceinline__ int of(float f, uint32_t key) const {
-    if (lo) return (int)((hi - key) >> shift);
-    const float x = f == top ? 0.0f : (top - f) * scale;
-    return x < kBins - 1 ? (int)x : x >= kBins - 1 ? kBins - 1 : 0;  // NaN (a scale of inf or 0): 0
-  }
+  // 2^23 + the distance below top in bins: its bits are the bin's number, and NaN and infinities compare as deep.
+  __device__ __forceinline__ float place(float f) const { return fmaf(top - f, scale, 8388608.0f); }
+  static __device__ __forceinline__ int bin(float place) { return __float_as_int(place) - 0x4b000000; }
+  __device__ __forceinline__ int of_key(uint32_t key) const { return (int)((hi - key) >> shift); }
   // The weight of a bin's middle, for estimates.
   __device__ __forceinline__ float middle(int b, float per_nat) const {
-    if (!lo) return __expf(-((float)b + 0.5f) / kBinsPerNat);
+    if (!lo) return __expf(-(float)b / kBinsPerNat);
     const uint32_t k = hi - min(hi - lo, ((uint32_t)b << shift) + ((1u << shift) >> 1));
     const float x = (top - logit_of(k)) * per_nat;
     return x > 0.0f ? __expf(-x) : 1.0f;
+  }
+  __device__ __forceinline__ void whole_row(uint32_t top_key) {
+    lo = 1, hi = top_key, shift = 0;
+    while (((hi - lo) >> shift) >= kBins) ++shift;
   }
 };
 
@@ -254,35 +287,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const int top_k = p.top_k ? p.top_k[row] : p.d_top_k;
   if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
 
-  // 1. The largest logit and its lowest index, as the pair (key, ~index).
-  u64 best = 0;
-  {
-    float f_best = -INFINITY;
-    int at = -1;
-    rd.each(v0, v1, [&](float f, int i) {
-      if (f > f_best) f_best = f, at = i;
-    });
-    best = (u64)key_of(f_best) << 32 | (0xffffffffu - (unsigned)at);
-#pragma unroll
-    for (int m = 16; m; m >>= 1) {
-      const u64 o = __shfl_xor_sync(0xffffffffu, best, m);
-      best = o > best ? o : best;
-    }
-    if (lane == 0) sm.scratch[warp] = best;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) best = sm.scratch[i] > best ? sm.scratch[i] : best;
-    if (threadIdx.x == 0) sm.best = best;
-    cl.sync();
-    for (int i = 0; i < C; ++i) {
-      const u64 o = *cl.map_shared_rank(&sm.best, i);
-      best = o > best ? o : best;
-    }
-  }
-  const uint32_t top_key = (uint32_t)(best >> 32);
+  // 1. The largest logit.
+  uint32_t top_key = key_of(rd.largest(v0, v1));
+  top_key = __reduce_max_sync(0xffffffffu, top_key);
+  if (threadIdx.x == 0) sm.key_max = 0, sm.key_min = 0xffffffffu;
+  __syncthreads();
+  if (lane == 0) atomicMax(&sm.key_max, top_key);
+  cl.sync();
+  for (int i = 0; i < C; ++i) top_key = max(top_key, *cl.map_shared_rank(&sm.key_max, i));
   if (top_key == 0 || !(t > 0.0f)) {
+    const float top = top_key ? logit_of(top_key) : 0.0f;
+    unsigned at = 0xffffffffu;  // its lowest index
+    if (top_key) rd.each(v0, v1, [&](float f, int i) {
+      if (f == top) at = min(at, (unsigned)i);
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) atomicMin(&sm.key_min, at);
+    cl.sync();
     if (rank == 0 && threadIdx.x == 0) {
-      p.token[row] = top_key ? (int)(0xffffffffu - (uint32_t)best) : -1;
+      for (int i = 0; i < C; ++i) at = min(at, *cl.map_shared_rank(&sm.key_min, i));
+      p.token[row] = (int)at;  // none: -1
       if (p.prob) p.prob[row] = top_key ? 1.0f : 0.0f;
       if (p.kept) p.kept[row] = top_key ? 1 : 0;
     }
@@ -310,6 +334,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   if (by_k || by_p) {
     Bins bins;
     bins.top = wt.top, bins.scale = kBinsPerNat / t, bins.lo = bins.hi = 0, bins.shift = 0;
+    const bool by_value = fabsf(wt.top) < INFINITY && bins.scale > 0.0f && bins.scale < INFINITY;
+    if (!by_value) bins.whole_row(top_key);
     bool counting = by_k;
     unsigned n_above = 0;           // tokens above the interval
     u64 base = 0, span = 0;         // weight above it, in it (by weight)
@@ -324,22 +350,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       // The histogram of the interval.
       for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
       __syncthreads();
-      u64 w = 0;
-      unsigned deep = 0;
+      u64 w = 0, sum;
       const bool weigh = !counting && !known;
-      rd.each(v0, v1, [&](float f, int) {
-        const uint32_t k = key_of(f);
-        if (k == 0 || (bins.lo && (k < bins.lo || k > bins.hi))) return;
-        const int b = bins.of(f, k);
-        if (b == kBins - 1) ++deep;
-        else atomicAdd(&sm.hist[b], 1u);
-        if (weigh) w += wt.whole(f);
-      });
-      u64 sum;
-      block_incl(w, sm.scratch, &sum);
-      if (threadIdx.x == 0) sm.total = sum;
-      for (int m = 16; m; m >>= 1) deep += __shfl_xor_sync(0xffffffffu, deep, m);
-      if (lane == 0 && deep) atomicAdd(&sm.hist[kBins - 1], deep);
+      constexpr float kDeep = 8388608.0f + (kBins - 1);
+      if (bins.lo) {
+        rd.each(v0, v1, [&](float f, int) {
+          const uint32_t k = key_of(f);
+          if (k == 0) return;
+          if (weigh) w += wt.whole(f);
+          if (k >= bins.lo && k <= bins.hi) atomicAdd(&sm.hist[bins.of_key(k)], 1u);
+        });
+      } else if (weigh) {
+        rd.each(v0, v1, [&](float f, int) {
+          if (!(f > -INFINITY)) return;
+          w += wt.whole(f);
+          const float at = bins.place(f);
+          if (at < kDeep) atomicAdd(&sm.hist[Bins::bin(at)], 1u);
+        });
+      } else {
+        rd.each(v0, v1, [&](float f, int) {
+          const float at = bins.place(f);
+          if (at < kDeep) atomicAdd(&sm.hist[Bins::bin(at)], 1u);
+        });
+      }
+      if (weigh) {
+        block_incl(w, sm.scratch, &sum);
+        if (threadIdx.x == 0) sm.total = sum;
+      }
       cl.sync();
       unsigned cnt[kPer] = {};
       for (int i = 0; i < C; ++i) {
@@ -364,10 +401,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         before = incl;
       }
       __syncthreads();
-      if (counting && n_above + tokens < (unsigned)top_k) {  // fewer tokens than top_k
-        by_k = counting = false;
-        if (!by_p) break;
+      if (counting && n_above + tokens < (unsigned)top_k) {
         cl.sync();
+        if (!bins.lo) {  // top_k reaches below the counted bins
+          bins.whole_row(top_key);
+          continue;
+        }
+        by_k = counting = false;  // fewer tokens than top_k
+        bins.lo = by_value ? 0 : bins.lo;
+        if (!by_p) break;
         continue;
       }
       auto pop = [&](int a, int b) { return sm.cum[b] - (a ? sm.cum[a - 1] : 0u); };
@@ -417,18 +459,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         if (threadIdx.x == 0) sm.n_list = 0, sm.key_min = 0xffffffffu, sm.key_max = 0;
         __syncthreads();
         u64 above = 0, in = 0;
-        rd.each(v0, v1, [&](float f, int i) {
-          const uint32_t k = key_of(f);
-          if (k == 0 || (bins.lo && k < bins.lo)) return;
-          const int b = bins.lo && k > bins.hi ? -1 : bins.of(f, k);
+        auto take = [&](float f, int i, uint32_t k, int b) {
           if (b < b0) {
             if (need) above += wt.whole(f);
-          } else if (b <= b1) {
+          } else {
             if (!counting) in += wt.whole(f);
             if (gather) sm.list[atomicAdd(&sm.n_list, 1u)] = (u64)k << 32 | (0xffffffffu - (unsigned)i);
             else atomicMin(&sm.key_min, k), atomicMax(&sm.key_max, k);
           }
-        });
+        };
+        if (bins.lo) {
+          rd.each(v0, v1, [&](float f, int i) {
+            const uint32_t k = key_of(f);
+            if (k < bins.lo) return;
+            const int b = k > bins.hi ? -1 : bins.of_key(k);
+            if (b <= b1) take(f, i, k, b);
+          });
+        } else {
+          const float limit = 8388608.0f + (float)b1;
+          rd.each(v0, v1, [&](float f, int i) {
+            const float at = bins.place(f);
+            if (at <= limit) take(f, i, key_of(f), Bins::bin(at));
+          });
+        }
         block_incl(above, sm.scratch, &sum);
         if (threadIdx.x == 0) sm.s_above = sum;
         block_incl(in, sm.scratch, &sum);
@@ -447,6 +500,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           bx = min(b0 - 1, by_weight((float)(e * ((double)(want - base) / (double)(above - base))), 0, b0 - 1));
           cl.sync();
           continue;
+        }
+        if (!counting && !bins.lo && b1 >= kBins - 2 && want > above + in) {  // below the counted bins
+          bins.whole_row(top_key);
+          n_above = 0, base = span = 0;
+          cl.sync();
+          break;
         }
         if (!counting && want > above + in) {  // further down
           const float e = estimate(b1);
@@ -477,7 +536,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           }
           if (found && by_p && each) ties = (unsigned)min((u64)ties, (want - above + each - 1) / each);
           if (!found) {  // top-p's border lies above top-k's: find it by weight, from the whole row
-            counting = false, known = true, base = span = 0, n_above = 0, bins.lo = 0;
+            counting = false, known = true, base = span = 0, n_above = 0;
+            if (by_value) bins.lo = 0;
+            else bins.whole_row(top_key);
           }
           cl.sync();
           break;
@@ -569,7 +630,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         const Verdict v = *cl.map_shared_rank(&sm.verdict, 0);
         cl.sync();
         if (v.again) {
-          counting = false, known = true, base = span = 0, n_above = 0, bins.lo = 0;
+          counting = false, known = true, base = span = 0, n_above = 0;
+          if (by_value) bins.lo = 0;
+          else bins.whole_row(top_key);
           total = v.total, want = want_of(total);
         } else {
           key = v.key, ties = v.ties, found = true;
@@ -585,18 +648,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const float x = wt.top + t * logf(min_p) - (0.01f * t + 1e-6f * fabsf(wt.top));
     if (x == x) far = fminf(x, wt.top);
   }
+  const float at_key = key ? logit_of(key) : __int_as_float(0x7fffffff);  // none: NaN
+  const float low = fmaxf(fmaxf(key ? at_key : -INFINITY, far), -3.402823466e38f);  // tokens below are not kept
   {
     Sums s{0, 0, 0};
     rd.each(v0, v1, [&](float f, int) {
-      const uint32_t k = key_of(f);
-      if (k == 0 || k < key || f < far) return;
-      if (k == key) {
+      if (!(f >= low)) return;
+      if (f == at_key) {
         ++s.ties;
         return;
       }
       double a, b;
       wt.parts(f, a, b);
-      if (min_p > 0.0f && !passes(k, a * b * wt.unit)) return;
+      if (min_p > 0.0f && f != wt.top && a * b * wt.unit < (double)min_p) return;
       s.w += (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - 0x4330000000000000ull;
       ++s.n;
     });
@@ -646,18 +710,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       if (v + lane < v1) rd.load(v + lane, f);
       unsigned eq = 0;
 #pragma unroll
-      for (int k = 0; k < VE; ++k) eq += key && key_of(f[k]) == key;
+      for (int k = 0; k < VE; ++k) eq += f[k] == at_key;
       const unsigned eq_incl = warp_incl(eq);
       unsigned my_tie = tie + eq_incl - eq;
       u64 q[VE], part = 0;
 #pragma unroll
       for (int k = 0; k < VE; ++k) {
-        const uint32_t kk = key_of(f[k]);
         q[k] = 0;
-        if (kk == 0 || kk < key || f[k] < far) continue;
-        if (kk == key) {
+        if (!(f[k] >= low)) continue;
+        if (f[k] == at_key) {
           if (my_tie++ < ties) q[k] = tie_w;
-        } else if (!(min_p > 0.0f) || passes(kk, wt.weight(f[k]))) {
+        } else if (!(min_p > 0.0f) || f[k] == wt.top || !(wt.weight(f[k]) < (double)min_p)) {
           q[k] = wt.whole(f[k]);
         }
         part += q[k];
