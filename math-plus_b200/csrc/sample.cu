@@ -5,13 +5,16 @@
 // All three filters keep a prefix of the tokens ranked by (logit descending, index ascending), so the kept
 // set is "every token above a threshold logit, and the first r tokens equal to it", and no row is sorted:
 //   1. the largest logit;
-//   2. a histogram of counts over 4096 bins of T / 128 below it finds the bin where the ranks reach top_k, or
-//      estimates the one where the weights reach top_p of their total;
-//   3. the tokens of that bin and the bins above it (at most 2048; else the bin alone) are gathered and sorted,
-//      and the border is found among them exactly, with the exact weight of what lies above. A bin of more
-//      than 2048 tokens is cut again, by the bits of its logits; an estimate that was off moves on.
-//   4. Where the gathered tokens are the whole kept set (any usual top_k, a narrow top_p) the draw is among them.
-//      Else every warp sums the kept weights of its stretch of the row, and the one that the draw falls into
+//   2. a bound below the border: for a small top_k, the least over the CTAs of their (top_k / CTAs)-th largest of the
+//      256 threads' maxima, since top_k tokens reach it for sure. Else a histogram of counts over 8192 bins of
+//      T / 256 below the largest gives the bin where the ranks reach top_k or, with the weights' exact total, an
+//      estimate of the one where the weights reach top_p of it;
+//   3. the tokens between the bound (or the bin, by weight the next one too) and what lies surely above are gathered
+//      (at most 256), the exact weight of those above is summed, and the border is found among the gathered, each
+//      compared with every other. An estimate that was off moves; a bin of more tokens is cut again, by the bits
+//      of its logits.
+//   4. Where the gathered tokens are the whole kept set (a small top_k, a narrow top_p) the draw is among them.
+//      Else every warp has the kept weight of its stretch of the row, and the one that the draw falls into
 //      walks its stretch.
 // Rows are read again by each step, from L1 or L2; HBM is read once.
 //
@@ -19,21 +22,23 @@
 // most 51), so that sums are exact whatever their order: the same row always gives the same token, and
 // the borders of top-p and of the drawn interval move by less than 1e-11 of the total.
 //
-// A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy: a few rows are bound by latency, many by the
-// f64 exponentials of the rows without top_k (about 12 double operations a token) and by the passes over L2.
+// A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy. A few rows are bound by latency (cluster
+// barriers and remote reads), many by the instructions per token of the passes, the f64 exponentials (10 double
+// operations each) of the rows without top_k above all.
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
 #include "mpc_internal.h"
+#include "sm100.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace mpc {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
-constexpr int kBins = 4096, kPer = kBins / kThreads, kList = 2048;
-constexpr float kBinsPerNat = 128.0f;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kBins = 8192, kList = kThreads, kSmallK = 192;
+constexpr float kBinsPerNat = 256.0f;
 
 struct SampleParams {
   const void *logits;
@@ -61,23 +66,42 @@ struct Sums {  // one warp's stretch: kept weight and tokens above the threshold
   u64 w;
   unsigned n, ties;
 };
+struct Share {  // one CTA's part of step 2: over its share of the bins, tokens and estimated weights; the weights' exact
+  u64 total;    // total over its stretch
+  unsigned n;
+  float e;
+};
+struct Border {  // a bin, the tokens above it and in it, the estimated weight above it
+  int bin;       // -1: none
+  unsigned over, pop;
+  float e;
+};
+struct Gathered {  // one CTA's part of step 3
+  u64 above, in;  // weight above the window; in it, where it is too much to be gathered
+  unsigned n, key_min, key_max;
+};
 struct Verdict {  // what the gathered tokens say
   u64 total;
   uint32_t key;
   unsigned ties;
-  int again;
+  int next;  // 0: the border is found; 1: it lies further up, 2: down; 3: top-p's lies above top-k's
 };
 struct Shared {
-  double table[32];  // 2^(i / 32)
-  unsigned hist[kBins];  // later the merged list
-  unsigned cum[kBins];   // tokens in bins 0..b, of the whole row
-  u64 list[kList];
-  u64 scratch[kWarps], s_above, s_in, total;
-  Sums sums[kWarps], all[kWarps * kMaxCluster];
-  float fscratch[kWarps];
-  unsigned n_list, key_min, key_max;
-  int b0, b1;
+  double table[32];  // 2^(i / 32 + shift)
+  u64 all[kList];    // the gathered tokens of the whole row
+  u64 list[kList];   // of this CTA's stretch
+  unsigned counts[kBins];
+  u64 scratch[kWarps];
+  Share share;
+  // Of each warp's and each CTA's share of the bins: where the border is reached; the last bin with tokens.
+  Border reached_in[kWarps], last_in[kWarps], reached[kMaxCluster], last[kMaxCluster];
+  unsigned warp_n[kWarps];
+  float warp_e[kWarps];
+  Gathered gathered;
   Verdict verdict;
+  Sums sums[kWarps], every[kWarps * kMaxCluster];
+  float largest[kThreads];
+  unsigned key_max, key_min, key_kth;
 };
 
 // Vectors of 16 bytes, aligned, over one row: vector v holds elements v * VE - mis ..+VE-1.
@@ -147,11 +171,15 @@ struct Reader {
     else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  // fn(logit, index) over vectors v0 + lane, + 32, ..; elements outside the row come as -inf.
+  // fn(16 logits, v) over vectors v0 + lane, + 32, ..: logit k is element element(v, k). All lanes of a warp go
+  // through as many batches; elements outside the row or the stretch come as -inf.
+  static constexpr int U = 16 / VE;
+  __device__ __forceinline__ int element(int v, int k) const { return index(v + 32 * (k / VE)) + k % VE; }
   template <typename Fn>
-  __device__ __forceinline__ void each(int v0, int v1, Fn fn) const {
-    constexpr int U = 16 / VE;  // 64 bytes (f32) or 32 in flight
-    for (int v = v0 + (threadIdx.x & 31); v < v1; v += 32 * U) {
+  __device__ __forceinline__ void batches(int v0, int v1, Fn fn) const {
+    const int lane = threadIdx.x & 31;
+    for (int w = v0; w < v1; w += 32 * U) {
+      const int v = w + lane;
       float f[U][VE];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -160,47 +188,62 @@ struct Reader {
 #pragma unroll
           for (int k = 0; k < VE; ++k) f[u][k] = -INFINITY;
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < VE; ++k) fn(f[u][k], index(v + 32 * u) + k);
+      fn(reinterpret_cast<const float(&)[16]>(f), v);
     }
+  }
+  template <typename Fn>
+  __device__ __forceinline__ void each(int v0, int v1, Fn fn) const {  // fn(logit, index)
+    batches(v0, v1, [&](const float(&f)[16], int v) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) fn(f[k], element(v, k));
+    });
   }
 };
 
 // w = 2^(y), y = (l - top) log2(e) / T, as 2^n * 2^(i / 32) * 2^r with |r| <= 1/64: the second from a table, the
-// last by its series to r^5 (the next term is below 3e-15).
+// last by its series to r^4 (the next term is below 1.3e-12 and changes sign with r).
+constexpr u64 kMagicBits = 0x4330000000000000ull;  // 2^52: the nearest whole number of a sum with it is in its low bits
 struct Weights {
   double c, unit;  // log2(e) / T; 2^-shift
-  float top;
-  int shift;
+  float top, floor;
+  bool plain;  // logits below `floor` weigh nothing, and clamping to it is safe
   const double *table;
-  __device__ __forceinline__ void parts(float f, double &s, double &p) const {
+  __device__ __forceinline__ void of(double y, double &s, double &p) const {
     constexpr double L = 0.69314718055994530942;
-    double y = f == top ? 0.0 : ((double)f - (double)top) * c;
-    y = fmax(y, -1000.0);  // also for NaN: logits below an infinite one
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
     const double t = fma(y, 32.0, magic);
     const int k = __double2loint(t);
     const double r = fma(t - magic, -1.0 / 32, y);
-    p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
-    p = fma(p, r, L * L * L / 6);
+    p = fma(r, L * L * L * L / 24, L * L * L / 6);
     p = fma(p, r, L * L / 2);
     p = fma(p, r, L);
     p = fma(p, r, 1.0);
     const double e = table[k & 31];
-    s = __hiloint2double(__double2hiint(e) + ((k >> 5) + shift) * (1 << 20), __double2loint(e));
+    s = __hiloint2double(__double2hiint(e) + ((k & ~31) << 15), __double2loint(e));
+  }
+  __device__ __forceinline__ void parts(float f, double &s, double &p) const {
+    const double y = f == top ? 0.0 : ((double)f - (double)top) * c;
+    of(fmax(y, -900.0), s, p);  // fmax also for NaN: logits below an infinite one
   }
   __device__ __forceinline__ double weight(float f) const {
     double s, p;
     parts(f, s, p);
     return s * p * unit;
   }
-  // The nearest whole number of units: below 2^52, so it appears in the low bits next to 2^52.
+  // The nearest whole number of units: below 2^52.
   __device__ __forceinline__ u64 whole(float f) const {
     double s, p;
     parts(f, s, p);
-    return (u64)__double_as_longlong(fma(s, p, 4503599627370496.0)) - 0x4330000000000000ull;
+    return (u64)__double_as_longlong(fma(s, p, 4503599627370496.0)) - kMagicBits;
+  }
+  // The same, for any f (0 for NaN and -inf), where `plain`.
+  __device__ __forceinline__ void parts_any(float f, double &s, double &p) const {
+    of(((double)fmaxf(f, floor) - (double)top) * c, s, p);
+  }
+  __device__ __forceinline__ u64 whole_any(float f) const {
+    double s, p;
+    parts_any(f, s, p);
+    return (u64)__double_as_longlong(fma(s, p, 4503599627370496.0)) - kMagicBits;
   }
 };
 
@@ -232,18 +275,11 @@ __device__ __forceinline__ T block_incl(T v, T *sm, T *all) {
   return v + before;
 }
 
-// Sorts n2 (a power of two) numbers in shared memory, descending or ascending.
-__device__ void sort(u64 *a, int n2, bool descending) {
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j; j >>= 1) {
-      __syncthreads();
-      for (int q = threadIdx.x; q < n2 / 2; q += kThreads) {
-        const int i = (q & ~(j - 1)) << 1 | (q & (j - 1)), l = i + j;
-        const u64 x = a[i], y = a[l];
-        if ((x < y) == (((i & k) == 0) == descending)) a[i] = y, a[l] = x;
-      }
-    }
-  __syncthreads();
+// counts[bin] + 1 where `at` is below `end`, without a branch; counts0 is the shared address less the bits of 2^23.
+__device__ __forceinline__ void count_if(uint32_t counts0, float at, float end) {
+  asm volatile("{\n .reg .pred p;\n setp.lt.f32 p, %1, %2;\n @p red.shared.add.u32 [%0], 1;\n}\n" ::"r"(
+                   counts0 + 4 * (uint32_t)__float_as_int(at)),
+               "f"(at), "f"(end));
 }
 
 // The histogram's bins: by value below the largest logit (the last bin is not used: what lies deeper is not
@@ -254,7 +290,6 @@ struct Bins {
   int shift;
   // 2^23 + the distance below top in bins: its bits are the bin's number, and NaN and infinities compare as deep.
   __device__ __forceinline__ float place(float f) const { return fmaf(top - f, scale, 8388608.0f); }
-  static __device__ __forceinline__ int bin(float place) { return __float_as_int(place) - 0x4b000000; }
   __device__ __forceinline__ int of_key(uint32_t key) const { return (int)((hi - key) >> shift); }
   // The weight of a bin's middle, for estimates.
   __device__ __forceinline__ float middle(int b, float per_nat) const {
@@ -269,12 +304,12 @@ struct Bins {
   }
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
+template <int DT, int C>
+__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared &sm = *reinterpret_cast<Shared *>(raw);
   const auto cl = cg::this_cluster();
-  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int rank = (int)cl.block_rank();
   const int row = blockIdx.x / C, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Reader<DT> rd;
   rd.set(p.logits, row * p.stride, p.vocab);
@@ -285,16 +320,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const float top_p = p.top_p ? p.top_p[row] : p.d_top_p;
   const float min_p = p.min_p ? p.min_p[row] : p.d_min_p;
   const int top_k = p.top_k ? p.top_k[row] : p.d_top_k;
-  if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  if (threadIdx.x < 32) sm.table[threadIdx.x] = ldexp(exp2(threadIdx.x / 32.0), p.shift);
+
+  Weights wt;
+  wt.c = 1.4426950408889634074 / (double)t;
+  wt.unit = ldexp(1.0, -p.shift);
+  wt.table = sm.table;
 
   // 1. The largest logit.
-  uint32_t top_key = key_of(rd.largest(v0, v1));
+  const float largest = rd.largest(v0, v1);
+  uint32_t top_key = key_of(largest);
+  bool by_k = top_k > 0 && top_k < p.vocab;
+  bool quick = by_k && top_k <= kSmallK;
+  if (quick) sm.largest[threadIdx.x] = largest;
   top_key = __reduce_max_sync(0xffffffffu, top_key);
-  if (threadIdx.x == 0) sm.key_max = 0, sm.key_min = 0xffffffffu;
+  if (threadIdx.x == 0) sm.key_max = sm.key_kth = 0, sm.key_min = 0xffffffffu;
   __syncthreads();
   if (lane == 0) atomicMax(&sm.key_max, top_key);
+  if (quick) {  // the thread whose maximum has rank ceil(top_k / C) - 1 of the CTA's
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < kThreads; ++i) above += sm.largest[i] > largest || (sm.largest[i] == largest && i < (int)threadIdx.x);
+    if (above == (top_k + C - 1) / C - 1) sm.key_kth = key_of(largest);
+  }
   cl.sync();
-  for (int i = 0; i < C; ++i) top_key = max(top_key, *cl.map_shared_rank(&sm.key_max, i));
+  // Lane i reads CTA i: one remote latency.
+  top_key = __reduce_max_sync(0xffffffffu, lane < C ? *cl.map_shared_rank(&sm.key_max, lane) : 0u);
+  const uint32_t bound = __reduce_min_sync(0xffffffffu, lane < C ? *cl.map_shared_rank(&sm.key_kth, lane) : 0xffffffffu);
   if (top_key == 0 || !(t > 0.0f)) {
     const float top = top_key ? logit_of(top_key) : 0.0f;
     unsigned at = 0xffffffffu;  // its lowest index
@@ -313,331 +365,363 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     cl.sync();  // nobody reads a CTA that has gone
     return;
   }
-  Weights wt;
   wt.top = logit_of(top_key);
-  wt.c = 1.4426950408889634074 / (double)t;
-  wt.shift = p.shift;
-  wt.unit = ldexp(1.0, -p.shift);
-  wt.table = sm.table;
+  wt.floor = wt.top - 46.0f * t;  // 2^-66
+  wt.plain = wt.top - wt.floor >= 40.0f * t && wt.floor >= -3.402823466e38f;  // not where t is lost next to top
   const float u = fminf(fmaxf(p.u[row], 0.0f), 1.0f);
   auto draw_of = [&](u64 total) {
     const u64 d = (u64)__double2ll_rd((double)u * (double)total);
     return d < total ? d : total - 1;
   };
-  auto passes = [&](uint32_t key, double w) { return key == top_key || !(w < (double)min_p); };
+  // Whether a kept token passes min_p.
+  auto passes = [&](float f) { return !(min_p > 0.0f) || f == wt.top || !(wt.weight(f) < (double)min_p); };
+  bool summed = false;  // the warps' sums are those of the tokens above the window, whose own are in the lists
+  u64 add_up = 0;
+  Sums s{0, 0, 0};
 
   // 2., 3. The threshold: keys above `key` are kept, and the first `ties` tokens of that key.
   uint32_t key = 0;
   unsigned ties = 0;
-  bool by_k = top_k > 0 && top_k < p.vocab;
   const bool by_p = top_p < 1.0f;
   if (by_k || by_p) {
     Bins bins;
     bins.top = wt.top, bins.scale = kBinsPerNat / t, bins.lo = bins.hi = 0, bins.shift = 0;
     const bool by_value = fabsf(wt.top) < INFINITY && bins.scale > 0.0f && bins.scale < INFINITY;
     if (!by_value) bins.whole_row(top_key);
+    quick = quick && bound;
     bool counting = by_k;
-    unsigned n_above = 0;           // tokens above the interval
-    u64 base = 0, span = 0;         // weight above it, in it (by weight)
-    u64 total = 0, want = 0;        // by weight: ranks before which less than `want` lies are kept
-    bool known = false;             // total is
+    unsigned n_above = 0;     // tokens above the interval
+    u64 base = 0;             // their weight
+    u64 total = 0, want = 0;  // by weight: ranks before which less than `want` lies are kept
+    bool known = false;       // total and want are
+    float factor = 0.0f;      // by weight: estimated over exact weight, as last seen (0: not yet)
+    int b_min = 0, b_max = kBins - 1;  // by weight: the border's bin is in here
+    bool alone = false;                // the window is the border's bin alone
     auto want_of = [&](u64 sum) {
       const double lim = top_p > 0.0f ? (double)top_p * (double)sum : 0.0;
       const u64 w = (u64)__double2ll_ru(lim);
       return w < 1 ? 1 : w > sum ? sum : w;
     };
+    auto whole_interval = [&] {
+      n_above = 0, base = 0, bins.lo = 0, factor = 0.0f, b_min = 0, b_max = kBins - 1;
+      if (!by_value) bins.whole_row(top_key);
+    };
     for (bool found = false; !found;) {
-      // The histogram of the interval.
-      for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
+      Border at{-1, 0, 0, 0.0f};
+      u64 sum = 0;
+      int b0 = 0, b1 = 0;
+      bool gather = true;
+      unsigned outside = 0;  // tokens above the window
+      if (threadIdx.x == 0) sm.gathered = Gathered{0, 0, 0, 0xffffffffu, 0};
+      if (!quick) {
+        // The histogram of the interval.
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sm.counts[i] = 0;
+        __syncthreads();
+        constexpr float kDeep = 8388608.0f + (kBins - 1);
+        const uint32_t counts0 = smem_u32(sm.counts) - 4u * 0x4b000000u;
+        const bool weigh = !counting && !known;
+        u64 w = 0;
+        if (bins.lo) {
+          rd.each(v0, v1, [&](float f, int) {
+            const uint32_t k = key_of(f);
+            if (weigh && k) w += wt.whole(f);
+            if (k >= bins.lo && k <= bins.hi) atomicAdd(&sm.counts[bins.of_key(k)], 1u);
+          });
+        } else if (weigh && wt.plain) {
+          rd.batches(v0, v1, [&](const float(&f)[16], int) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              count_if(counts0, bins.place(f[k]), kDeep);
+              w += wt.whole_any(f[k]);
+            }
+          });
+        } else {
+          rd.batches(v0, v1, [&](const float(&f)[16], int) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) count_if(counts0, bins.place(f[k]), kDeep);
+          });
+          if (weigh) rd.each(v0, v1, [&](float f, int) { w += f > -INFINITY ? wt.whole(f) : 0; });
+        }
+        if (weigh) block_incl(w, sm.scratch, &sum);
+        cl.sync();
+        // CTA r adds up the C histograms over its share of the bins, each warp over consecutive ones.
+        constexpr int steps = kBins / kThreads / C;
+        const int first = (rank * kWarps + warp) * 32 * steps + lane;
+        const float per_nat = 1.0f / t;
+        unsigned mine = 0, over = n_above;
+        float mine_e = 0.0f, before_e = 0.0f, all_e = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < steps; ++j) {
+          unsigned n = 0;
+#pragma unroll
+          for (int i = 0; i < C; ++i) n += cl.map_shared_rank(sm.counts, i)[first + 32 * j];
+          if (C > 1) sm.counts[first + 32 * j] = n;  // nobody else reads this share here
+          mine += n;
+          if (!counting && n) mine_e += (float)n * bins.middle(first + 32 * j, per_nat);
+        }
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        for (int i = 16; i; i >>= 1) mine_e += __shfl_xor_sync(0xffffffffu, mine_e, i);
+        if (lane == 0) sm.warp_n[warp] = mine, sm.warp_e[warp] = mine_e, sm.reached_in[warp].bin = sm.last_in[warp].bin = -1;
+        __syncthreads();
+        unsigned n_share = 0;
+        float e_share = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+          if (i < warp) over += sm.warp_n[i], before_e += sm.warp_e[i];
+          n_share += sm.warp_n[i], e_share += sm.warp_e[i];
+        }
+        if (threadIdx.x == 0) sm.share = Share{sum, n_share, e_share};
+        cl.sync();
+        {
+          Share x{0, 0, 0.0f};
+          if (lane < C) x = *cl.map_shared_rank(&sm.share, lane);
+          over += __shfl_sync(0xffffffffu, warp_incl(x.n) - x.n, rank);
+          if (!counting) {
+            const float ei = warp_incl(x.e);
+            before_e += __shfl_sync(0xffffffffu, ei - x.e, rank);
+            all_e = __shfl_sync(0xffffffffu, ei, 31);
+            if (!known) total = __shfl_sync(0xffffffffu, warp_incl(x.total), 31), want = want_of(total), known = true;
+            // What is estimated adds up to the total, unless the interval is a part of the row.
+            if (factor == 0.0f) factor = base || bins.lo > 1 ? (float)wt.unit : (float)((double)all_e / (double)total);
+          }
+        }
+        const float goal = (float)(want - base) * factor;
+        if (!counting || (over < (unsigned)top_k && over + mine >= (unsigned)top_k))
+          for (int j = 0; j < steps; ++j) {
+            const int bin = first + 32 * j;
+            const unsigned n = sm.counts[bin], ni = warp_incl(n);
+            const float e = !counting && n ? (float)n * bins.middle(bin, per_nat) : 0.0f, ei = counting ? 0.0f : warp_incl(e);
+            const bool in = n && bin >= b_min && bin <= b_max;
+            const unsigned hit = __ballot_sync(0xffffffffu, in && (counting ? over + ni >= (unsigned)top_k : before_e + ei >= goal));
+            const unsigned some = __ballot_sync(0xffffffffu, in);
+            const Border mark{bin, over + ni - n, n, before_e + ei - e};
+            if (hit && lane == __ffs(hit) - 1) sm.reached_in[warp] = mark;
+            if (some && lane == 31 - __clz(some)) sm.last_in[warp] = mark;
+            if (hit) break;
+            over += __shfl_sync(0xffffffffu, ni, 31);
+            before_e += __shfl_sync(0xffffffffu, ei, 31);
+          }
+        __syncthreads();
+        if (threadIdx.x < C) {  // thread i tells CTA i
+          Border reached{-1, 0, 0, 0.0f}, last = reached;
+          for (int i = kWarps - 1; i >= 0; --i) {
+            if (sm.reached_in[i].bin >= 0) reached = sm.reached_in[i];
+            if (last.bin < 0) last = sm.last_in[i];
+          }
+          Shared *const to = cl.map_shared_rank(&sm, threadIdx.x);
+          to->reached[rank] = reached, to->last[rank] = last;
+        }
+        cl.sync();
+        // The first bin where the border is reached; by weight, where the estimate misses it, the last.
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          if (at.bin < 0 && sm.reached[i].bin >= 0) at = sm.reached[i];
+        }
+        if (at.bin < 0 && !counting)
+#pragma unroll
+          for (int i = 0; i < C; ++i)
+            if (sm.last[i].bin >= 0) at = sm.last[i];
+        if (at.bin < 0) {
+          if (!bins.lo) {  // the border lies below the counted bins
+            whole_interval();
+            bins.whole_row(top_key);
+            continue;
+          }
+          if (!counting) break;  // not reached: the weights add up to the total
+          by_k = counting = false;  // fewer tokens than top_k
+          whole_interval();
+          if (!by_p) break;
+          continue;
+        }
+        // The window: the border's bin, by weight the next one too, and all above where they are few.
+        gather = at.pop <= kList;
+        b1 = counting || !gather || alone || at.bin == kBins - 1 ? at.bin : at.bin + 1;
+        b0 = gather && at.over - n_above + 2 * at.pop <= kList ? 0 : at.bin;
+        outside = b0 ? at.over : n_above;
+      }
       __syncthreads();
-      u64 w = 0, sum;
-      const bool weigh = !counting && !known;
-      constexpr float kDeep = 8388608.0f + (kBins - 1);
+      const bool need = outside && (by_p || gather);  // the weight of those above it
+      s = Sums{0, 0, 0}, add_up = 0;
+      u64 in_window = 0;
+      auto note = [&](float f) {  // a token above the window
+        const u64 x = wt.whole(f);
+        add_up += x;
+        if (passes(f)) s.w += x, ++s.n;
+      };
+      auto note_any = [&](float f, bool is) {  // the same without a branch
+        double a, b;
+        wt.parts_any(f, a, b);
+        const u64 x = is ? (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - kMagicBits : 0;
+        add_up += x;
+        if (!(min_p > 0.0f) || f == wt.top || !(a * b * wt.unit < (double)min_p)) s.w += x, s.n += is;
+      };
+      auto take = [&](float f, int i) {  // one in the window
+        const uint32_t k = key_of(f);
+        if (gather) {
+          const unsigned place = atomicAdd(&sm.gathered.n, 1u);
+          if (place < kList) sm.list[place] = (u64)k << 32 | (0xffffffffu - (unsigned)i);
+        } else {
+          atomicMin(&sm.gathered.key_min, k), atomicMax(&sm.gathered.key_max, k);
+          if (!counting) in_window += wt.whole(f);
+        }
+      };
       if (bins.lo) {
-        rd.each(v0, v1, [&](float f, int) {
+        rd.each(v0, v1, [&](float f, int i) {
           const uint32_t k = key_of(f);
-          if (k == 0) return;
-          if (weigh) w += wt.whole(f);
-          if (k >= bins.lo && k <= bins.hi) atomicAdd(&sm.hist[bins.of_key(k)], 1u);
-        });
-      } else if (weigh) {
-        rd.each(v0, v1, [&](float f, int) {
-          if (!(f > -INFINITY)) return;
-          w += wt.whole(f);
-          const float at = bins.place(f);
-          if (at < kDeep) atomicAdd(&sm.hist[Bins::bin(at)], 1u);
+          if (k < bins.lo) return;
+          const int b = k > bins.hi ? -1 : bins.of_key(k);
+          if (b > b1) return;
+          if (b >= b0) take(f, i);
+          else if (need) note(f);
         });
       } else {
-        rd.each(v0, v1, [&](float f, int) {
-          const float at = bins.place(f);
-          if (at < kDeep) atomicAdd(&sm.hist[Bins::bin(at)], 1u);
+        // place() of a token, or its negative for the bound: above the window below `a`, in it up to `z`.
+        const float g_top = quick ? 0.0f : wt.top, g_scale = quick ? 1.0f : bins.scale, g_bias = quick ? 0.0f : 8388608.0f;
+        const float a = quick ? -INFINITY : g_bias + (float)b0, z = quick ? -logit_of(bound) : g_bias + (float)b1;
+        rd.batches(v0, v1, [&](const float(&f)[16], int v) {
+          float x[16], least = INFINITY;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[k] = fmaf(g_top - f[k], g_scale, g_bias), least = fminf(least, x[k]);
+          if (!__any_sync(0xffffffffu, least <= z)) return;
+          if (need && wt.plain) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) note_any(f[k], x[k] < a);
+          } else if (need) {
+            for (int k = 0; k < 16; ++k)
+              if (x[k] < a) note(f[k]);
+          }
+          if (least <= z)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (x[k] <= z && !(x[k] < a)) take(f[k], rd.element(v, k));
         });
       }
-      if (weigh) {
-        block_incl(w, sm.scratch, &sum);
-        if (threadIdx.x == 0) sm.total = sum;
-      }
-      cl.sync();
-      unsigned cnt[kPer] = {};
-      for (int i = 0; i < C; ++i) {
-        const uint4 *h = reinterpret_cast<const uint4 *>(cl.map_shared_rank(sm.hist, i) + threadIdx.x * kPer);
-#pragma unroll
-        for (int j = 0; j < kPer / 4; ++j) {
-          const uint4 x = h[j];
-          cnt[4 * j] += x.x, cnt[4 * j + 1] += x.y, cnt[4 * j + 2] += x.z, cnt[4 * j + 3] += x.w;
-        }
-        if (weigh) total += *cl.map_shared_rank(&sm.total, i);
-      }
-      if (weigh) known = true, want = want_of(total), span = total;
-      unsigned mine = 0, tokens;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) mine += cnt[j];
-      unsigned before = block_incl(mine, reinterpret_cast<unsigned *>(sm.scratch), &tokens) - mine;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const unsigned incl = before + cnt[j];
-        sm.cum[threadIdx.x * kPer + j] = incl;
-        if (counting && n_above + before < (unsigned)top_k && n_above + incl >= (unsigned)top_k) sm.b1 = threadIdx.x * kPer + j;
-        before = incl;
-      }
+      u64 sum_in = 0;
+      sum = 0;
+      if (need) block_incl(add_up, sm.scratch, &sum);
+      if (!gather && !counting) block_incl(in_window, sm.scratch, &sum_in);
       __syncthreads();
-      if (counting && n_above + tokens < (unsigned)top_k) {
-        cl.sync();
-        if (!bins.lo) {  // top_k reaches below the counted bins
-          bins.whole_row(top_key);
-          continue;
-        }
-        by_k = counting = false;  // fewer tokens than top_k
-        bins.lo = by_value ? 0 : bins.lo;
-        if (!by_p) break;
-        continue;
-      }
-      auto pop = [&](int a, int b) { return sm.cum[b] - (a ? sm.cum[a - 1] : 0u); };
-      // The bin where the estimated weights reach `goal`, within [lo, hi], into sm.b1.
-      auto by_weight = [&](float goal, int lo, int hi) {
-        float e[kPer], part = 0.0f, all;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int b = threadIdx.x * kPer + j;
-          e[j] = (float)pop(b, b) * bins.middle(b, 1.0f / t);
-          part += e[j];
-        }
-        float upto = block_incl(part, sm.fscratch, &all) - part;
-        if (threadIdx.x == 0) sm.b1 = hi;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          upto += e[j];
-          if (upto >= goal) atomicMin(&sm.b1, threadIdx.x * kPer + j);
-        }
-        __syncthreads();
-        const int b = max(sm.b1, lo);
-        __syncthreads();
-        return b;
+      if (threadIdx.x == 0) sm.gathered.above = sum, sm.gathered.in = sum_in;
+      cl.sync();
+      Gathered got{0, 0, 0, 0xffffffffu, 0};
+      if (lane < C) got = *cl.map_shared_rank(&sm.gathered, lane);
+      const unsigned listed = warp_incl(got.n);  // in CTAs 0..lane
+      const unsigned m = __shfl_sync(0xffffffffu, listed, 31);
+      const u64 above = __shfl_sync(0xffffffffu, warp_incl(got.above), 31);
+      const u64 in = __shfl_sync(0xffffffffu, warp_incl(got.in), 31);
+      const uint32_t kmin = __reduce_min_sync(0xffffffffu, got.key_min), kmax = __reduce_max_sync(0xffffffffu, got.key_max);
+      // The estimate missed the border: look on above or below the window, by what the exact weights say.
+      auto move = [&](bool up) {
+        if (up) b_max = at.bin - 1;
+        else b_min = b1 + 1;
+        if (above > base && at.e > 0.0f) factor = at.e / (float)(above - base);
       };
-      auto estimate = [&](int upto) {  // of the weights of bins 0..upto
-        float part = 0.0f, all;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int b = threadIdx.x * kPer + j;
-          if (b <= upto) part += (float)pop(b, b) * bins.middle(b, 1.0f / t);
-        }
-        block_incl(part, sm.fscratch, &all);
-        return all;
-      };
-      int bx;
-      if (counting) bx = sm.b1;
-      else bx = by_weight(span ? estimate(kBins - 1) * (float)((double)(want - base) / (double)span) : (float)((double)(want - base) * wt.unit), 0, kBins - 1);
-      for (;;) {
-        // The window [b0, b1]: all down to the border where the list holds that, else the bins next to it.
-        int b1 = counting ? bx : min(bx + 1, kBins - 1);
-        int b0 = pop(0, b1) <= kList ? 0 : counting ? bx : max(bx - 1, 0);
-        if (pop(b0, b1) > kList) b0 = b1 = bx;
-        const bool gather = pop(b0, b1) <= kList;
-        const bool need = !counting || by_p;
-        __syncthreads();
-        if (threadIdx.x == 0) sm.n_list = 0, sm.key_min = 0xffffffffu, sm.key_max = 0;
-        __syncthreads();
-        u64 above = 0, in = 0;
-        auto take = [&](float f, int i, uint32_t k, int b) {
-          if (b < b0) {
-            if (need) above += wt.whole(f);
-          } else {
-            if (!counting) in += wt.whole(f);
-            if (gather) sm.list[atomicAdd(&sm.n_list, 1u)] = (u64)k << 32 | (0xffffffffu - (unsigned)i);
-            else atomicMin(&sm.key_min, k), atomicMax(&sm.key_max, k);
-          }
-        };
-        if (bins.lo) {
-          rd.each(v0, v1, [&](float f, int i) {
-            const uint32_t k = key_of(f);
-            if (k < bins.lo) return;
-            const int b = k > bins.hi ? -1 : bins.of_key(k);
-            if (b <= b1) take(f, i, k, b);
-          });
-        } else {
-          const float limit = 8388608.0f + (float)b1;
-          rd.each(v0, v1, [&](float f, int i) {
-            const float at = bins.place(f);
-            if (at <= limit) take(f, i, key_of(f), Bins::bin(at));
-          });
-        }
-        block_incl(above, sm.scratch, &sum);
-        if (threadIdx.x == 0) sm.s_above = sum;
-        block_incl(in, sm.scratch, &sum);
-        if (threadIdx.x == 0) sm.s_in = sum;
-        cl.sync();
-        above = in = 0;
-        uint32_t kmin = 0xffffffffu, kmax = 0;
-        for (int i = 0; i < C; ++i) {
-          above += *cl.map_shared_rank(&sm.s_above, i);
-          in += *cl.map_shared_rank(&sm.s_in, i);
-          kmin = min(kmin, *cl.map_shared_rank(&sm.key_min, i));
-          kmax = max(kmax, *cl.map_shared_rank(&sm.key_max, i));
-        }
-        if (!counting && want <= above) {  // the border lies further up
-          const float e = estimate(b0 - 1);
-          bx = min(b0 - 1, by_weight((float)(e * ((double)(want - base) / (double)(above - base))), 0, b0 - 1));
+      if (!gather) {
+        if (!counting && (want <= above || want > above + in)) {
+          move(want <= above);
           cl.sync();
           continue;
         }
-        if (!counting && !bins.lo && b1 >= kBins - 2 && want > above + in) {  // below the counted bins
-          bins.whole_row(top_key);
-          n_above = 0, base = span = 0;
-          cl.sync();
-          break;
-        }
-        if (!counting && want > above + in) {  // further down
-          const float e = estimate(b1);
-          bx = by_weight((float)(e * ((double)(want - base) / (double)(above + in - base))), b1 + 1, kBins - 1);
-          cl.sync();
-          continue;
-        }
-        const unsigned over = n_above + (b0 ? sm.cum[b0 - 1] : 0u);  // tokens above the window
-        if (!gather && kmin < kmax) {  // cut the window again by its keys
+        if (kmin < kmax) {  // cut the bin again by its keys
           bins.lo = kmin, bins.hi = kmax, bins.shift = 0;
           while (((kmax - kmin) >> bins.shift) >= kBins) ++bins.shift;
-          n_above = over, base = above, span = counting ? 0 : in;
+          n_above = outside, base = above, factor = 0.0f, b_min = 0, b_max = kBins - 1;
           cl.sync();
-          break;
+          continue;
         }
-        if (!gather) {  // more equal logits than the list holds
-          const u64 each = wt.whole(logit_of(kmin));
-          key = kmin;
-          found = true;
-          if (counting) {
-            ties = (unsigned)top_k - over;
-            if (by_p) {
-              total = above + ties * each, want = want_of(total);
-              if (want <= above) found = false;
-            }
-          } else {
-            ties = pop(b0, b1);
-          }
-          if (found && by_p && each) ties = (unsigned)min((u64)ties, (want - above + each - 1) / each);
-          if (!found) {  // top-p's border lies above top-k's: find it by weight, from the whole row
-            counting = false, known = true, base = span = 0, n_above = 0;
-            if (by_value) bins.lo = 0;
-            else bins.whole_row(top_key);
-          }
-          cl.sync();
-          break;
+        // More equal logits than the list holds.
+        const u64 each = wt.whole(logit_of(kmin));
+        key = kmin, ties = at.pop, found = true;
+        if (counting) {
+          ties = (unsigned)top_k - outside;
+          if (by_p) total = above + ties * each, want = want_of(total);
         }
-        // The first CTA sorts the gathered tokens and finds the border among them.
-        if (rank == 0) {
-          u64 *const all = reinterpret_cast<u64 *>(sm.hist);
-          int n = 0;
-          for (int i = 0; i < C; ++i) {
-            const int m = (int)*cl.map_shared_rank(&sm.n_list, i);
-            const u64 *from = cl.map_shared_rank(sm.list, i);
-            for (int j = threadIdx.x; j < m; j += kThreads) all[n + j] = from[j];
-            n += m;
+        if (counting && by_p && want <= above) {  // top-p's border lies above top-k's
+          found = false, counting = false, known = true;
+          whole_interval();
+        } else if (by_p && each) {
+          ties = (unsigned)min((u64)ties, (want - above + each - 1) / each);
+        }
+        cl.sync();
+        continue;
+      }
+      // The first CTA finds the border among the gathered tokens.
+      if (rank == 0) {
+        for (int i = warp; i < C; i += kWarps) {
+          const int end = (int)__shfl_sync(0xffffffffu, listed, i), size = (int)__shfl_sync(0xffffffffu, got.n, i);
+          const u64 *from = cl.map_shared_rank(sm.list, i);
+          for (int j = lane; j < size; j += 32)
+            if (end - size + j < kList) sm.all[end - size + j] = from[j];
+        }
+        const int lim = counting ? min((int)m, (int)((unsigned)top_k - outside)) : (int)m;
+        Verdict v{0, 0, 0, 0};
+        if (m <= kList) {
+          // A thread per token, its rank and the weight before it by comparison with every other.
+          u64 *const q = reinterpret_cast<u64 *>(sm.counts);
+          u64 me = 0, w = 0;
+          __syncthreads();
+          if (threadIdx.x < m) {
+            me = sm.all[threadIdx.x];
+            w = wt.whole(logit_of((uint32_t)(me >> 32)));
+            q[threadIdx.x] = w;
           }
-          int n2 = 32;
-          while (n2 < n) n2 <<= 1;
-          for (int j = n + threadIdx.x; j < n2; j += kThreads) all[j] = 0;
-          sort(all, n2, true);
-          const int lim = counting ? min(n, (int)((unsigned)top_k - over)) : n;
-          // Thread i weighs ranks 4i ..+3.
-          u64 q[kList / kThreads], part = 0;
-          const int r0 = threadIdx.x * (kList / kThreads);
-#pragma unroll
-          for (int j = 0; j < kList / kThreads; ++j) {
-            q[j] = r0 + j < lim && by_p ? wt.whole(logit_of((uint32_t)(all[r0 + j] >> 32))) : 0;
-            part += q[j];
-          }
-          u64 upto = block_incl(part, sm.scratch, &sum) - part;
-          u64 goal = want;
-          bool again = false;
-          if (counting && by_p) {
-            total = above + sum, goal = want_of(total);
-            again = goal <= above;
-          }
-          unsigned kept = 0;
-          upto += above;
-#pragma unroll
-          for (int j = 0; j < kList / kThreads; ++j) {
-            kept += r0 + j < lim && (!by_p || upto < goal);
-            upto += q[j];
-          }
-          unsigned n_kept;
-          block_incl(kept, reinterpret_cast<unsigned *>(sm.scratch), &n_kept);
-          if (over == 0) {
-            // 4. The kept set is among the gathered tokens: min-p, then the draw in the order of the indices.
-            kept = 0;
-            for (unsigned j = threadIdx.x; j < n_kept; j += kThreads) {
-              const uint32_t k = (uint32_t)(all[j] >> 32);
-              kept += passes(k, wt.weight(logit_of(k)));
+          __syncthreads();
+          int rank_of = 0;
+          u64 before = above;
+          for (int j = 0; j < (int)m; ++j)
+            if (sm.all[j] > me) ++rank_of, before += q[j];
+          const bool in_k = threadIdx.x < m && rank_of < lim;
+          block_incl(in_k ? w : 0, sm.scratch, &sum);
+          if (counting && by_p) total = above + sum, want = want_of(total);
+          v.total = total;
+          v.next = !by_p ? 0 : want <= above ? (counting ? 3 : 1) : want > above + sum ? 2 : 0;
+          bool kept = in_k && (!by_p || before < want);
+          if (outside == 0 && v.next == 0) {
+            // 4. The kept set is among the gathered tokens: the draw in the order of the indices.
+            const float f = logit_of((uint32_t)(me >> 32));
+            kept = kept && passes(f);
+            if (threadIdx.x < m && !kept) q[threadIdx.x] = 0;
+            const int n_kept = __syncthreads_count(kept);
+            u64 upto = 0;
+            sum = 0;
+            for (int j = 0; j < (int)m; ++j) {
+              const u64 x = q[j];
+              sum += x;
+              if ((uint32_t)sm.all[j] > (uint32_t)me) upto += x;  // a lower index
             }
-            block_incl(kept, reinterpret_cast<unsigned *>(sm.scratch), &n_kept);
-            n2 = 32;
-            while (n2 < (int)n_kept) n2 <<= 1;
-            for (int j = threadIdx.x; j < n2; j += kThreads) {
-              const u64 x = all[j];
-              all[j] = j < (int)n_kept ? (u64)(0xffffffffu - (uint32_t)x) << 32 | x >> 32 : ~0ull;
-            }
-            sort(all, n2, false);
-            part = 0;
-#pragma unroll
-            for (int j = 0; j < kList / kThreads; ++j) {
-              q[j] = r0 + j < (int)n_kept ? wt.whole(logit_of((uint32_t)all[r0 + j])) : 0;
-              part += q[j];
-            }
-            upto = block_incl(part, sm.scratch, &sum) - part;
             const u64 d = draw_of(sum);
-#pragma unroll
-            for (int j = 0; j < kList / kThreads; ++j) {
-              if (upto <= d && d < upto + q[j]) {
-                const u64 x = all[r0 + j];
-                p.token[row] = (int32_t)(x >> 32);
-                if (p.prob) p.prob[row] = (float)(wt.weight(logit_of((uint32_t)x)) / ((double)sum * wt.unit));
-              }
-              upto += q[j];
+            if (kept && upto <= d && d < upto + w) {
+              p.token[row] = (int32_t)(0xffffffffu - (uint32_t)me);
+              if (p.prob) p.prob[row] = (float)(wt.weight(f) / ((double)sum * wt.unit));
             }
-            if (threadIdx.x == 0 && p.kept) p.kept[row] = (int32_t)n_kept;
-          } else if (threadIdx.x == 0) {
-            Verdict v;
-            v.total = total, v.again = again, v.key = 0, v.ties = 0;
-            if (!again) {
-              v.key = (uint32_t)(all[n_kept - 1] >> 32);
-              for (int j = (int)n_kept - 1; j >= 0 && (uint32_t)(all[j] >> 32) == v.key; --j) ++v.ties;
-            }
-            sm.verdict = v;
+            if (threadIdx.x == 0 && p.kept) p.kept[row] = n_kept;
+          } else if (v.next == 0) {
+            const int n_kept = __syncthreads_count(kept);
+            if (kept && rank_of == n_kept - 1) sm.key_min = (uint32_t)(me >> 32);
+            __syncthreads();
+            v.key = sm.key_min;
+            v.ties = (unsigned)__syncthreads_count(kept && (uint32_t)(me >> 32) == v.key);
           }
         }
-        cl.sync();
-        if (over == 0) return;  // the first CTA has drawn
-        const Verdict v = *cl.map_shared_rank(&sm.verdict, 0);
-        cl.sync();
-        if (v.again) {
-          counting = false, known = true, base = span = 0, n_above = 0;
-          if (by_value) bins.lo = 0;
-          else bins.whole_row(top_key);
-          total = v.total, want = want_of(total);
-        } else {
-          key = v.key, ties = v.ties, found = true;
-        }
-        break;
+        if (threadIdx.x == 0) sm.verdict = v;
+      }
+      cl.sync();
+      if (m > kList) {  // more than expected: by a histogram, or without the next bin
+        if (!quick) alone = true;
+        quick = false;
+        continue;
+      }
+      const Verdict v = *cl.map_shared_rank(&sm.verdict, 0);
+      cl.sync();
+      quick = false;
+      if (v.next == 0 && outside == 0) return;  // the first CTA has drawn
+      if (v.next == 0) {
+        key = v.key, ties = v.ties, found = summed = true;
+      } else if (v.next == 3) {  // top-p's border lies above top-k's
+        counting = false, known = true, total = v.total, want = want_of(total);
+        whole_interval();
+      } else {
+        move(v.next == 1);
       }
     }
   }
@@ -651,19 +735,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   const float at_key = key ? logit_of(key) : __int_as_float(0x7fffffff);  // none: NaN
   const float low = fmaxf(fmaxf(key ? at_key : -INFINITY, far), -3.402823466e38f);  // tokens below are not kept
   {
-    Sums s{0, 0, 0};
-    rd.each(v0, v1, [&](float f, int) {
-      if (!(f >= low)) return;
-      if (f == at_key) {
-        ++s.ties;
-        return;
-      }
+    auto add = [&](float f) {
       double a, b;
       wt.parts(f, a, b);
       if (min_p > 0.0f && f != wt.top && a * b * wt.unit < (double)min_p) return;
-      s.w += (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - 0x4330000000000000ull;
+      s.w += (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - kMagicBits;
       ++s.n;
-    });
+    };
+    if (!summed) s = Sums{0, 0, 0};
+    if (summed) {
+      // The tokens above the window are in the sums; the kept ones in it follow below.
+    } else if (!key && !(min_p > 0.0f) && wt.plain) {  // the whole row
+      rd.each(v0, v1, [&](float f, int) {
+        s.w += wt.whole_any(f);
+        s.n += f > -INFINITY;
+      });
+    } else {
+      rd.each(v0, v1, [&](float f, int) {
+        if (!(f >= low)) return;
+        if (f == at_key) ++s.ties;
+        else add(f);
+      });
+    }
 #pragma unroll
     for (int m = 16; m; m >>= 1) {
       s.w += __shfl_xor_sync(0xffffffffu, s.w, m);
@@ -672,18 +765,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     }
     if (lane == 0) sm.sums[warp] = s;
   }
+  if (summed) {
+    __syncthreads();
+    for (unsigned j = threadIdx.x; j < sm.gathered.n; j += kThreads) {
+      const u64 x = sm.list[j];
+      const float f = logit_of((uint32_t)(x >> 32));
+      if (!(f >= low)) continue;
+      Sums &to = sm.sums[(((int)(0xffffffffu - (uint32_t)x) + rd.mis) / Reader<DT>::VE - rank * per_cta) / per_warp];
+      if (f == at_key) atomicAdd(&to.ties, 1u);
+      else if (passes(f)) atomicAdd(&to.w, wt.whole(f)), atomicAdd(&to.n, 1u);
+    }
+  }
   cl.sync();
-  for (int i = threadIdx.x; i < C * kWarps; i += kThreads) sm.all[i] = cl.map_shared_rank(sm.sums, i / kWarps)[i % kWarps];
+  for (int i = threadIdx.x; i < C * kWarps; i += kThreads) sm.every[i] = cl.map_shared_rank(sm.sums, i / kWarps)[i % kWarps];
   __syncthreads();
   const u64 tie_w = key ? wt.whole(logit_of(key)) : 0;
-  if (key && !passes(key, wt.weight(logit_of(key)))) ties = 0;
+  if (key && !passes(at_key)) ties = 0;
   // Each warp walks the stretches up to its own, lane by lane of 32.
   u64 total = 0, before = 0, mine = 0;
   unsigned kept = 0, tie_before = 0, tie_at = 0;
   const int self = rank * kWarps + warp;
   for (int i0 = 0; i0 < C * kWarps; i0 += 32) {
     Sums s{0, 0, 0};
-    if (i0 + lane < C * kWarps) s = sm.all[i0 + lane];
+    if (i0 + lane < C * kWarps) s = sm.every[i0 + lane];
     const unsigned tie_incl = tie_at + warp_incl(s.ties), tie_excl = tie_incl - s.ties;
     const unsigned take = min(ties, tie_incl) - min(ties, tie_excl);
     const u64 w = s.w + take * tie_w, incl = total + warp_incl(w);
@@ -720,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         if (!(f[k] >= low)) continue;
         if (f[k] == at_key) {
           if (my_tie++ < ties) q[k] = tie_w;
-        } else if (!(min_p > 0.0f) || f[k] == wt.top || !(wt.weight(f[k]) < (double)min_p)) {
+        } else if (passes(f[k])) {
           q[k] = wt.whole(f[k]);
         }
         part += q[k];
@@ -745,26 +849,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   cl.sync();
 }
 
-template <int DT>
-int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
+template <int DT, int C>
+int launch_cluster(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
   static bool configured[64] = {};
   const int ord = dev->ordinal & 63;
   if (!configured[ord]) {
-    MPC_CUDA(dev, cudaFuncSetAttribute(sample_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+    MPC_CUDA(dev, cudaFuncSetAttribute(sample_kernel<DT, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
     configured[ord] = true;
   }
-  // CTAs per row: up to two for every SM, of at least 2048 tokens.
-  int c = 1;
-  while (c < kMaxCluster && (long long)rows * c < 2ll * dev->prop.multiProcessorCount && p.vocab >= 2 * c * 2048) c *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)rows * c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sizeof(Shared), cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)rows * C), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sizeof(Shared), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)c, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = C, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  MPC_CUDA(dev, cudaLaunchKernelEx(&cfg, sample_kernel<DT>, p));
+  MPC_CUDA(dev, cudaLaunchKernelEx(&cfg, sample_kernel<DT, C>, p));
   dev->launches++;
   return MPC_OK;
+}
+
+// CTAs per row: up to the four that an SM holds, of at least 1024 tokens.
+template <int DT>
+int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
+  int c = 1;
+  while (c < kMaxCluster && (long long)rows * c <= 2ll * dev->prop.multiProcessorCount && p.vocab >= 2 * c * 1024) c *= 2;
+  if (c == 8) return launch_cluster<DT, 8>(dev, p, rows, st);
+  if (c == 4) return launch_cluster<DT, 4>(dev, p, rows, st);
+  if (c == 2) return launch_cluster<DT, 2>(dev, p, rows, st);
+  return launch_cluster<DT, 1>(dev, p, rows, st);
 }
 
 }  // namespace
