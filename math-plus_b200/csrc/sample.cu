@@ -88,8 +88,9 @@ struct Verdict {  // what the gathered tokens say
 };
 struct Shared {
   double table[32];  // 2^(i / 32 + shift)
-  u64 all[kList];    // the gathered tokens of the whole row
-  u64 list[kList];   // of this CTA's stretch
+  u64 list[kList];  // the gathered tokens of this CTA's stretch
+  u64 all[kList];   // of the row (the first CTA)
+  u64 q[kThreads];
   unsigned counts[kBins];
   u64 scratch[kWarps];
   Share share;
@@ -100,7 +101,11 @@ struct Shared {
   Gathered gathered;
   Verdict verdict;
   Sums sums[kWarps], every[kWarps * kMaxCluster];
-  float largest[kThreads];
+  union {
+    float largest[kThreads];
+    float queue[kWarps][544];  // a batch of 512 and 31 that wait
+  };
+  unsigned waiting[kWarps];
   unsigned key_max, key_min, key_kth;
 };
 
@@ -305,7 +310,7 @@ struct Bins {
 };
 
 template <int DT, int C>
-__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared &sm = *reinterpret_cast<Shared *>(raw);
   const auto cl = cg::this_cluster();
@@ -375,6 +380,12 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   };
   // Whether a kept token passes min_p.
   auto passes = [&](float f) { return !(min_p > 0.0f) || f == wt.top || !(wt.weight(f) < (double)min_p); };
+  float far = -INFINITY, sure = -INFINITY;  // below `far` w < min_p, from `sure` on not, f32's rounding allowed for
+  if (min_p > 0.0f) {
+    const float x = wt.top + t * logf(min_p), slack = 0.01f * t + 1e-6f * fabsf(wt.top);
+    sure = wt.top;
+    if (x - slack == x - slack) far = fminf(x - slack, wt.top), sure = fminf(x + slack, wt.top);
+  }
   bool summed = false;  // the warps' sums are those of the tokens above the window, whose own are in the lists
   u64 add_up = 0;
   Sums s{0, 0, 0};
@@ -397,12 +408,14 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
     float factor = 0.0f;      // by weight: estimated over exact weight, as last seen (0: not yet)
     int b_min = 0, b_max = kBins - 1;  // by weight: the border's bin is in here
     bool alone = false;                // the window is the border's bin alone
+    bool counted = false;              // the interval's histogram is at hand
     auto want_of = [&](u64 sum) {
       const double lim = top_p > 0.0f ? (double)top_p * (double)sum : 0.0;
       const u64 w = (u64)__double2ll_ru(lim);
       return w < 1 ? 1 : w > sum ? sum : w;
     };
     auto whole_interval = [&] {
+      counted = counted && !bins.lo;
       n_above = 0, base = 0, bins.lo = 0, factor = 0.0f, b_min = 0, b_max = kBins - 1;
       if (!by_value) bins.whole_row(top_key);
     };
@@ -415,33 +428,37 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       if (threadIdx.x == 0) sm.gathered = Gathered{0, 0, 0, 0xffffffffu, 0};
       if (!quick) {
         // The histogram of the interval.
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sm.counts[i] = 0;
-        __syncthreads();
-        constexpr float kDeep = 8388608.0f + (kBins - 1);
-        const uint32_t counts0 = smem_u32(sm.counts) - 4u * 0x4b000000u;
         const bool weigh = !counting && !known;
         u64 w = 0;
-        if (bins.lo) {
-          rd.each(v0, v1, [&](float f, int) {
-            const uint32_t k = key_of(f);
-            if (weigh && k) w += wt.whole(f);
-            if (k >= bins.lo && k <= bins.hi) atomicAdd(&sm.counts[bins.of_key(k)], 1u);
-          });
-        } else if (weigh && wt.plain) {
-          rd.batches(v0, v1, [&](const float(&f)[16], int) {
+        const bool fresh = !counted || weigh;
+        if (fresh) {
+          for (int i = threadIdx.x; i < kBins; i += kThreads) sm.counts[i] = 0;
+          __syncthreads();
+          constexpr float kDeep = 8388608.0f + (kBins - 1);
+          const uint32_t counts0 = smem_u32(sm.counts) - 4u * 0x4b000000u;
+          if (bins.lo) {
+            rd.each(v0, v1, [&](float f, int) {
+              const uint32_t k = key_of(f);
+              if (weigh && k) w += wt.whole(f);
+              if (k >= bins.lo && k <= bins.hi) atomicAdd(&sm.counts[bins.of_key(k)], 1u);
+            });
+          } else if (weigh && wt.plain) {
+            rd.batches(v0, v1, [&](const float(&f)[16], int) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              count_if(counts0, bins.place(f[k]), kDeep);
-              w += wt.whole_any(f[k]);
-            }
-          });
-        } else {
-          rd.batches(v0, v1, [&](const float(&f)[16], int) {
+              for (int k = 0; k < 16; ++k) {
+                count_if(counts0, bins.place(f[k]), kDeep);
+                w += wt.whole_any(f[k]);
+              }
+            });
+          } else {
+            rd.batches(v0, v1, [&](const float(&f)[16], int) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) count_if(counts0, bins.place(f[k]), kDeep);
-          });
-          if (weigh) rd.each(v0, v1, [&](float f, int) { w += f > -INFINITY ? wt.whole(f) : 0; });
+              for (int k = 0; k < 16; ++k) count_if(counts0, bins.place(f[k]), kDeep);
+            });
+            if (weigh) rd.each(v0, v1, [&](float f, int) { w += f > -INFINITY ? wt.whole(f) : 0; });
+          }
         }
+        counted = true;
         if (weigh) block_incl(w, sm.scratch, &sum);
         cl.sync();
         // CTA r adds up the C histograms over its share of the bins, each warp over consecutive ones.
@@ -453,9 +470,13 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
 #pragma unroll 4
         for (int j = 0; j < steps; ++j) {
           unsigned n = 0;
+          if (C > 1 && fresh) {
 #pragma unroll
-          for (int i = 0; i < C; ++i) n += cl.map_shared_rank(sm.counts, i)[first + 32 * j];
-          if (C > 1) sm.counts[first + 32 * j] = n;  // nobody else reads this share here
+            for (int i = 0; i < C; ++i) n += cl.map_shared_rank(sm.counts, i)[first + 32 * j];
+            sm.counts[first + 32 * j] = n;  // nobody else reads this share here
+          } else {
+            n = sm.counts[first + 32 * j];
+          }
           mine += n;
           if (!counting && n) mine_e += (float)n * bins.middle(first + 32 * j, per_nat);
         }
@@ -525,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
           if (!bins.lo) {  // the border lies below the counted bins
             whole_interval();
             bins.whole_row(top_key);
+            counted = false;
             continue;
           }
           if (!counting) break;  // not reached: the weights add up to the total
@@ -541,19 +563,15 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
       }
       __syncthreads();
       const bool need = outside && (by_p || gather);  // the weight of those above it
+      const bool few = outside < (unsigned)p.vocab / 16;
+      if (lane == 0) sm.waiting[warp] = 0;
+      __syncwarp();
       s = Sums{0, 0, 0}, add_up = 0;
       u64 in_window = 0;
       auto note = [&](float f) {  // a token above the window
         const u64 x = wt.whole(f);
         add_up += x;
         if (passes(f)) s.w += x, ++s.n;
-      };
-      auto note_any = [&](float f, bool is) {  // the same without a branch
-        double a, b;
-        wt.parts_any(f, a, b);
-        const u64 x = is ? (u64)__double_as_longlong(fma(a, b, 4503599627370496.0)) - kMagicBits : 0;
-        add_up += x;
-        if (!(min_p > 0.0f) || f == wt.top || !(a * b * wt.unit < (double)min_p)) s.w += x, s.n += is;
       };
       auto take = [&](float f, int i) {  // one in the window
         const uint32_t k = key_of(f);
@@ -579,23 +597,55 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
         const float g_top = quick ? 0.0f : wt.top, g_scale = quick ? 1.0f : bins.scale, g_bias = quick ? 0.0f : 8388608.0f;
         const float a = quick ? -INFINITY : g_bias + (float)b0, z = quick ? -logit_of(bound) : g_bias + (float)b1;
         rd.batches(v0, v1, [&](const float(&f)[16], int v) {
-          float x[16], least = INFINITY;
+          auto at = [&](int k) { return fmaf(g_top - f[k], g_scale, g_bias); };
+          float least = INFINITY;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = fmaf(g_top - f[k], g_scale, g_bias), least = fminf(least, x[k]);
+          for (int k = 0; k < 16; ++k) least = fminf(least, at(k));
           if (!__any_sync(0xffffffffu, least <= z)) return;
-          if (need && wt.plain) {
+          if (need && few) {  // they queue up for exponentials of 32 at once
 #pragma unroll
-            for (int k = 0; k < 16; ++k) note_any(f[k], x[k] < a);
-          } else if (need) {
-            for (int k = 0; k < 16; ++k)
-              if (x[k] < a) note(f[k]);
+            for (int k = 0; k < 16; ++k) {
+              const float x = at(k);
+              if (x < a) sm.queue[warp][atomicAdd(&sm.waiting[warp], 1u)] = f[k];
+              else if (x <= z) take(f[k], rd.element(v, k));
+            }
+            __syncwarp();
+            unsigned n = sm.waiting[warp];
+            if (n >= 32) {
+              for (; n >= 32; n -= 32) note(sm.queue[warp][n - 32 + lane]);
+              __syncwarp();
+              if (lane == 0) sm.waiting[warp] = n;
+              __syncwarp();
+            }
+            return;
           }
-          if (least <= z)
+          if (need) {
+            if (wt.plain) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const u64 w = wt.whole_any(f[k]);
+                if (at(k) < a) {
+                  add_up += w;
+                  if (f[k] >= sure || (f[k] >= far && passes(f[k]))) s.w += w, ++s.n;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (at(k) < a) note(f[k]);
+            }
+            least = INFINITY;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) least = fminf(least, at(k) < a ? INFINITY : at(k));
+          }
+          if (least <= z) {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              if (x[k] <= z && !(x[k] < a)) take(f[k], rd.element(v, k));
+              if (at(k) <= z && !(at(k) < a)) take(f[k], rd.element(v, k));
+          }
         });
       }
+      if (lane < (int)sm.waiting[warp]) note(sm.queue[warp][lane]);
       u64 sum_in = 0;
       sum = 0;
       if (need) block_incl(add_up, sm.scratch, &sum);
@@ -623,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
           continue;
         }
         if (kmin < kmax) {  // cut the bin again by its keys
-          bins.lo = kmin, bins.hi = kmax, bins.shift = 0;
+          bins.lo = kmin, bins.hi = kmax, bins.shift = 0, counted = false;
           while (((kmax - kmin) >> bins.shift) >= kBins) ++bins.shift;
           n_above = outside, base = above, factor = 0.0f, b_min = 0, b_max = kBins - 1;
           cl.sync();
@@ -657,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
         Verdict v{0, 0, 0, 0};
         if (m <= kList) {
           // A thread per token, its rank and the weight before it by comparison with every other.
-          u64 *const q = reinterpret_cast<u64 *>(sm.counts);
+          u64 *const q = sm.q;
           u64 me = 0, w = 0;
           __syncthreads();
           if (threadIdx.x < m) {
@@ -727,11 +777,6 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleParams 
   }
 
   // 4. Every warp's kept weight, and the one that the draw falls into.
-  float far = -INFINITY;  // below it w < min_p for sure
-  if (min_p > 0.0f) {
-    const float x = wt.top + t * logf(min_p) - (0.01f * t + 1e-6f * fabsf(wt.top));
-    if (x == x) far = fminf(x, wt.top);
-  }
   const float at_key = key ? logit_of(key) : __int_as_float(0x7fffffff);  // none: NaN
   const float low = fmaxf(fmaxf(key ? at_key : -INFINITY, far), -3.402823466e38f);  // tokens below are not kept
   {
@@ -868,11 +913,12 @@ int launch_cluster(mpc_device *dev, const SampleParams &p, int rows, cudaStream_
   return MPC_OK;
 }
 
-// CTAs per row: up to the four that an SM holds, of at least 1024 tokens.
+// CTAs per row: more than the two that an SM holds, so that the rows under way at a time stay in L2 for the later
+// passes (256 rows of 131071 f32: 2, 4 and 8 CTAs 346, 242 and 232 us), and at least 1024 tokens each.
 template <int DT>
 int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
   int c = 1;
-  while (c < kMaxCluster && (long long)rows * c <= 2ll * dev->prop.multiProcessorCount && p.vocab >= 2 * c * 1024) c *= 2;
+  while (c < kMaxCluster && (long long)rows * c <= 4ll * dev->prop.multiProcessorCount && p.vocab >= 2 * c * 1024) c *= 2;
   if (c == 8) return launch_cluster<DT, 8>(dev, p, rows, st);
   if (c == 4) return launch_cluster<DT, 4>(dev, p, rows, st);
   if (c == 2) return launch_cluster<DT, 2>(dev, p, rows, st);
