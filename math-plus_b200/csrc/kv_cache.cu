@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kv_cache.cuh"
 #include "mpc_internal.h"
 
@@ -26,6 +28,19 @@ namespace mpc {
 namespace {
 
 constexpr int kThreads = 256;
+
+__device__ __forceinline__ void store_raw8(void *p, int dt, long long i, const Raw8 &x, bool zero) {
+  Raw8 y;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y.r[k] = zero ? 0u : x.r[k];
+  if (dt == MPC_F32) {
+    uint4 *q = reinterpret_cast<uint4 *>(static_cast<float *>(p) + i);
+    q[0] = make_uint4(y.r[0], y.r[1], y.r[2], y.r[3]);
+    q[1] = make_uint4(y.r[4], y.r[5], y.r[6], y.r[7]);
+  } else {
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(y.r[0], y.r[1], y.r[2], y.r[3]);
+  }
+}
 
 struct KvParams {
   void *pages[2];      // K, V
@@ -88,9 +103,47 @@ __device__ __forceinline__ bool locate(const KvParams &p, long long t, long long
   return true;
 }
 
-// One group of LPR lanes per token, walking the heads blockIdx.y, + gridDim.y, ..
-template <int LPR, bool VEC, bool APPEND>
+// The largest magnitude of a row's finite values, as f32 bits, over the LPR lanes of its group. Magnitudes compare as
+// their bits, two 16-bit ones at a time; a row with a NaN or an infinity (the largest bits of all) is gone through again.
+template <int LPR>
+__device__ __forceinline__ uint32_t row_amax(const Raw8 &v, int dt, bool mine) {
+  uint32_t m = 0, end;  // from `end` on: not finite
+  if (dt == MPC_F32) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, v.r[k] & 0x7fffffffu);
+    end = 0x7f800000u;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = __vmaxu2(m, v.r[k] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    end = dt == MPC_BF16 ? 0x7f80u : 0x7c00u;
+  }
+  if (!mine) m = 0;
+#pragma unroll
+  for (int i = LPR / 2; i; i >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, i));
+  if (__any_sync(0xffffffffu, m >= end)) {
+    m = 0;
+    if (mine) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t a = dt == MPC_F32 ? v.r[k] & 0x7fffffffu : (v.r[k >> 1] >> (16 * (k & 1))) & 0x7fffu;
+        if (a < end) m = max(m, a);
+      }
+    }
+#pragma unroll
+    for (int i = LPR / 2; i; i >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, i));
+  }
+  return dt == MPC_F32 ? m : dt == MPC_BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+
+// One group of LPR lanes per token, walking the heads blockIdx.y, + gridDim.y, .. With VEC the K and V rows of H heads
+// are loaded before any is used, whether the token is written or not.
+// DR, DP: the types of the rows and the pages; kAny: as the parameters say (the fixed ones save a third of the
+// instructions, which bound the 8-bit forms next to HBM).
+constexpr int kAny = -1;
+template <int LPR, bool VEC, int H, bool APPEND, int DR, int DP>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const KvParams p) {
+  const int dt_rows = DR == kAny ? p.dt_rows : DR, dt_pages = DP == kAny ? p.dt_pages : DP;
   const int lane = threadIdx.x % LPR;
   const int groups = kThreads / LPR;
   for (long long t0 = (long long)blockIdx.x * groups; t0 < p.n; t0 += (long long)gridDim.x * groups) {
@@ -99,47 +152,94 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(const KvParams p) {
     int off = 0;
     const bool live = t < p.n;
     const bool ok = live && locate(p, t, &page, &off, lane == 0 && blockIdx.y == 0);
-    for (int h = blockIdx.y; h < p.hk; h += gridDim.y) {
+    const long long row0 = page * p.hk * p.page_size + off;  // of head 0
+    const bool any = APPEND || p.n_pages > 0;                // an empty cache has no row to read in place of a bad one
+    const long long tt = live ? t : p.n - 1;
+    // This lane's 8 values of head h: rows_at + h * hs, pages_at + h * step.
+    long long rows_at[2], pages_at[2];
+    int step[2];
+    bool mine[2];
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int d = p.d[w];
-        const bool mine = lane * 8 < d;
-        const long long row = (page * p.hk + h) * p.page_size + off;
-        const long long at = row * d + lane * 8;
-        const long long src = t * p.ts[w] + h * p.hs[w] + lane * 8;
-        float x[8];
-        if constexpr (APPEND) {
+    for (int w = 0; w < 2; ++w) {
+      mine[w] = lane * 8 < p.d[w];
+      const int at = mine[w] ? lane * 8 : 0;
+      rows_at[w] = tt * p.ts[w] + at, pages_at[w] = row0 * p.d[w] + at, step[w] = p.page_size * p.d[w];
+    }
+    for (int h0 = blockIdx.y; h0 < p.hk; h0 += H * gridDim.y) {
+      Raw8 raw[H][2];
+      uint32_t byte[H][2];
+      if constexpr (VEC) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-          if (ok && mine) load8<VEC>(p.rows[w], p.dt_rows, src, d - lane * 8, x);
-          if (p.dt_pages == MPC_E4M3) {
-            uint32_t amax = 0;
+        for (int u = 0; u < H; ++u)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t a = __float_as_uint(x[k]) & 0x7fffffffu;
-              if (a < 0x7f800000u) amax = max(amax, a);
-            }
-#pragma unroll
-            for (int m = LPR / 2; m; m >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-            const int sb = scale_byte(amax);
-            const float inv = __uint_as_float((uint32_t)(254 - sb) << 23);  // 2^-(sb - 127): sb in 1..247
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] *= inv;
-            if (ok && lane == 0) p.scales[w][row] = (uint8_t)sb;
-          }
-          if (ok && mine) store8<VEC>(p.pages[w], p.dt_pages, at, d - lane * 8, x);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-          if (ok && mine) {
-            load8<VEC>(p.pages[w], p.dt_pages, at, d - lane * 8, x);
-            if (p.dt_pages == MPC_E4M3) {
-              const float s = scale_value(p.scales[w][row]);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) x[k] *= s;
+          for (int w = 0; w < 2; ++w) {
+            const int h = H == 1 ? h0 : min(h0 + u * (int)gridDim.y, p.hk - 1);
+            if (APPEND) {
+              load_raw8(p.rows[w], dt_rows, rows_at[w] + h * p.hs[w], raw[u][w]);
+            } else if (any) {
+              load_raw8(p.pages[w], dt_pages, pages_at[w] + (long long)h * step[w], raw[u][w]);
+              if (dt_pages == MPC_E4M3) byte[u][w] = p.scales[w][row0 + (long long)h * p.page_size];
             }
           }
-          if (live && mine) store8<VEC>(p.rows[w], p.dt_rows, src, d - lane * 8, x);
+      }
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        const int h = h0 + u * (int)gridDim.y;
+        if (H > 1 && h >= p.hk) break;  // the same for the whole block
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int n = p.d[w] - lane * 8;
+          const long long in_rows = rows_at[w] + h * p.hs[w], in_pages = pages_at[w] + (long long)h * step[w];
+          if constexpr (VEC) {
+            if (dt_pages == dt_rows) {  // as they are
+              if (APPEND ? ok && mine[w] : live && mine[w])
+                store_raw8(APPEND ? p.pages[w] : p.rows[w], dt_rows, APPEND ? in_pages : in_rows, raw[u][w], !ok);
+              continue;
+            }
+          }
+          float x[8];
+          if constexpr (APPEND) {
+            if constexpr (!VEC) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+              if (ok && mine[w]) load8<false>(p.rows[w], dt_rows, in_rows, n, x);
+            }
+            if (dt_pages == MPC_E4M3) {
+              uint32_t amax = 0;
+              if constexpr (VEC) {
+                amax = row_amax<LPR>(raw[u][w], dt_rows, mine[w]);
+                widen8(raw[u][w], dt_rows, x);
+              } else {
+                Raw8 v;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v.r[k] = __float_as_uint(x[k]);
+                amax = row_amax<LPR>(v, MPC_F32, mine[w]);
+              }
+              const int sb = scale_byte(amax);
+              const float inv = __uint_as_float((uint32_t)(254 - sb) << 23);  // 2^-(sb - 127): sb in 1..247
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] *= inv;
+              if (ok && lane == 0) p.scales[w][row0 + (long long)h * p.page_size] = (uint8_t)sb;
+            }
+            if (ok && mine[w]) store8<VEC>(p.pages[w], dt_pages, in_pages, n, x);
+          } else {
+            if constexpr (VEC) {
+              widen8(raw[u][w], dt_pages, x);
+              const float s = dt_pages == MPC_E4M3 ? scale_value(byte[u][w]) : 1.0f;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = ok ? x[k] * s : 0.0f;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+              if (ok && mine[w]) {
+                load8<false>(p.pages[w], dt_pages, in_pages, n, x);
+                const float s = dt_pages == MPC_E4M3 ? scale_value(p.scales[w][row0 + (long long)h * p.page_size]) : 1.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] *= s;
+              }
+            }
+            if (live && mine[w]) store8<VEC>(p.rows[w], dt_rows, in_rows, n, x);
+          }
         }
       }
     }
@@ -192,10 +292,30 @@ int kv_run(mpc_device *dev, const char *what, const mpc_kv_desc *c, void *k_page
   long long gy = want / bx;
   gy = gy > c->hk ? c->hk : gy;
   const dim3 grid(bx, (unsigned)(gy < 1 ? 1 : gy > 65535 ? 65535 : gy));
+  const bool two = vec && 2ll * grid.y <= c->hk;  // a block walks several heads: two at a time
   auto run = [&](auto kern) { kern<<<grid, kThreads, 0, st>>>(p); };
-  if (lpr == 8) vec ? run(kv_rows_kernel<8, true, APPEND>) : run(kv_rows_kernel<8, false, APPEND>);
-  else if (lpr == 16) vec ? run(kv_rows_kernel<16, true, APPEND>) : run(kv_rows_kernel<16, false, APPEND>);
-  else vec ? run(kv_rows_kernel<32, true, APPEND>) : run(kv_rows_kernel<32, false, APPEND>);
+  auto pick = [&](auto width) {
+    constexpr int LPR = decltype(width)::value;
+    auto fixed = [&](auto rows, auto pages) {
+      constexpr int R = decltype(rows)::value, P = decltype(pages)::value;
+      two ? run(kv_rows_kernel<LPR, true, 2, APPEND, R, P>) : run(kv_rows_kernel<LPR, true, 1, APPEND, R, P>);
+    };
+    using std::integral_constant;
+    const integral_constant<int, MPC_F32> f32;
+    const integral_constant<int, MPC_F16> f16;
+    const integral_constant<int, MPC_BF16> bf16;
+    const integral_constant<int, MPC_E4M3> e4m3;
+    const integral_constant<int, kAny> any;
+    if (!vec) run(kv_rows_kernel<LPR, false, 1, APPEND, kAny, kAny>);
+    else if (t->dtype == c->dtype) t->dtype == MPC_F32 ? fixed(f32, f32) : fixed(bf16, bf16);  // a copy: f16 alike
+    else if (c->dtype != MPC_E4M3) fixed(any, any);
+    else if (t->dtype == MPC_F32) fixed(f32, e4m3);
+    else if (t->dtype == MPC_F16) fixed(f16, e4m3);
+    else fixed(bf16, e4m3);
+  };
+  if (lpr == 8) pick(std::integral_constant<int, 8>());
+  else if (lpr == 16) pick(std::integral_constant<int, 16>());
+  else pick(std::integral_constant<int, 32>());
   dev->launches++;
   return check_launch(dev, what);
 }

@@ -96,27 +96,44 @@ __device__ __forceinline__ void store_f32(void *p, int dt, long long i, float v)
   }
 }
 
-// 8 values from index i of a row, as f32; with VEC the address is a multiple of 8 values.
+// 8 values from index i of a row as stored, and as f32; with VEC the address is a multiple of 8 values.
+struct Raw8 {
+  uint32_t r[8];
+};
+__device__ __forceinline__ void load_raw8(const void *p, int dt, long long i, Raw8 &x) {
+  if (dt == MPC_F32) {
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + i);
+    const uint4 a = q[0], b = q[1];
+    x.r[0] = a.x, x.r[1] = a.y, x.r[2] = a.z, x.r[3] = a.w, x.r[4] = b.x, x.r[5] = b.y, x.r[6] = b.z, x.r[7] = b.w;
+  } else if (dt == MPC_E4M3) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p) + i);
+    x.r[0] = v.x, x.r[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+    x.r[0] = v.x, x.r[1] = v.y, x.r[2] = v.z, x.r[3] = v.w;
+  }
+}
+__device__ __forceinline__ void widen8(const Raw8 &v, int dt, float (&x)[8]) {
+  if (dt == MPC_F32) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(v.r[k]);
+  } else if (dt == MPC_E4M3) {
+    e4m3x4_to_f32(v.r[0], x);
+    e4m3x4_to_f32(v.r[1], x + 4);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = dt == MPC_BF16 ? bf16x2_to_f32(v.r[k]) : f16x2_to_f32(v.r[k]);
+      x[2 * k] = f.x, x[2 * k + 1] = f.y;
+    }
+  }
+}
 template <bool VEC>
 __device__ __forceinline__ void load8(const void *p, int dt, long long i, int n, float (&x)[8]) {
   if constexpr (VEC) {
-    if (dt == MPC_F32) {
-      const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-      const float4 a = q[0], b = q[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else if (dt == MPC_E4M3) {
-      const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(p) + i);
-      e4m3x4_to_f32(v.x, x);
-      e4m3x4_to_f32(v.y, x + 4);
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = dt == MPC_BF16 ? bf16x2_to_f32(w[k]) : f16x2_to_f32(w[k]);
-        x[2 * k] = f.x, x[2 * k + 1] = f.y;
-      }
-    }
+    Raw8 v;
+    load_raw8(p, dt, i, v);
+    widen8(v, dt, x);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = k < n ? load_f32(p, dt, i + k) : 0.0f;
