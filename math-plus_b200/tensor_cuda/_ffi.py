@@ -62,6 +62,9 @@ class GemmDesc(C.Structure):
                 ("b_batch_stride", C.c_int64 * 4)]
 
 
+I64x2 = C.c_int64 * 2
+
+
 class KvDesc(C.Structure):
     """mpc_kv_desc: the shape and storage of a paged key/value cache."""
     _fields_ = [("n_pages", C.c_int64), ("page_size", C.c_int64), ("hk", C.c_int64), ("d", C.c_int64),
@@ -70,14 +73,14 @@ class KvDesc(C.Structure):
 
 class KvTokens(C.Structure):
     """mpc_kv_tokens: the dense rows of an append or a read."""
-    _fields_ = [("n", C.c_int64), ("n_seq", C.c_int64), ("max_pages", C.c_int64), ("k_stride", C.c_int64 * 2),
-                ("v_stride", C.c_int64 * 2), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+    _fields_ = [("n", C.c_int64), ("n_seq", C.c_int64), ("max_pages", C.c_int64), ("k_stride", I64x2),
+                ("v_stride", I64x2), ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
 class SdpaPagedDesc(C.Structure):
     """mpc_sdpa_paged_desc."""
-    _fields_ = [("b", C.c_int64), ("h", C.c_int64), ("max_pages", C.c_int64), ("q_stride", C.c_int64 * 2),
-                ("o_stride", C.c_int64 * 2), ("dtype", C.c_int32), ("scale", C.c_float)]
+    _fields_ = [("b", C.c_int64), ("h", C.c_int64), ("max_pages", C.c_int64), ("q_stride", I64x2),
+                ("o_stride", I64x2), ("dtype", C.c_int32), ("scale", C.c_float)]
 
 
 class SampleDesc(C.Structure):

@@ -754,29 +754,31 @@ class CudaBackend:
     # (kv_cache.py; no counterpart in the reference)
     def _mine(self, where: str, *ts) -> None:
         """Live tensors of this device."""
-        self._check_live(*ts)
         for t in ts:
-            if t is not None and t.backend.device is not self.device:
+            if t is None:
+                continue
+            if t.disposed:
+                raise RuntimeError("tensor-cuda: tensor used after dispose")
+            if t.backend is not self and t.backend.device is not self.device:
                 raise ValueError(f"tensor-cuda: {where}: tensor of another device (no implicit transfers)")
 
-    def _kv_tokens(self, where: str, cache, table: CudaTensor, pos: CudaTensor, seq: CudaTensor | None, n: int):
+    def _kv_places(self, where: str, cache, table: CudaTensor, pos: CudaTensor, seq: CudaTensor | None, n: int) -> None:
+        """Checks the cache, the table [n_seq, max_pages] and n tokens' positions and sequence indices."""
         self._mine(where, table, pos, seq)
-        if cache.backend.device is not self.device:
+        if cache.backend is not self and cache.backend.device is not self.device:
             raise ValueError(f"tensor-cuda: {where}: cache of another device (no implicit transfers)")
         if cache.disposed:
             raise RuntimeError(f"tensor-cuda: {where}: cache used after dispose")
-        for t, rank, name in ((table, 2, "table"), (pos, 1, "pos"), (seq, 1, "seq")):
-            if t is not None and (t.dtype != "i32" or len(t.shape) != rank):
-                raise TypeError(f"tensor-cuda: {where}: {name} is i32 of rank {rank}, got {t.dtype} "
-                                f"[{','.join(map(str, t.shape))}]")
+        if table.dtype != "i32" or pos.dtype != "i32" or len(table.shape) != 2 or len(pos.shape) != 1 or \
+                (seq is not None and (seq.dtype != "i32" or len(seq.shape) != 1)):
+            got = ", ".join(f"{t.dtype} [{','.join(map(str, t.shape))}]" for t in (table, pos, seq) if t is not None)
+            raise TypeError(f"tensor-cuda: {where}: the table is i32 of rank 2, positions, lengths and sequence indices "
+                            f"i32 of rank 1; got {got}")
         if pos.shape[0] != n or (seq is not None and seq.shape[0] != n):
             raise ValueError(f"tensor-cuda: {where}: {n} tokens, {pos.shape[0]} positions"
                              + (f", {seq.shape[0]} sequence indices" if seq is not None else ""))
         if seq is None and n > table.shape[0]:
             raise ValueError(f"tensor-cuda: {where}: {n} tokens for {table.shape[0]} sequences need seq")
-        tok = F.KvTokens()
-        tok.n, tok.n_seq, tok.max_pages = n, table.shape[0], table.shape[1]
-        return tok
 
     def kv_append(self, cache, k: CudaTensor, v: CudaTensor, table: CudaTensor, pos: CudaTensor,
                   seq: CudaTensor | None = None) -> None:
@@ -791,10 +793,7 @@ class CudaBackend:
                              f" for {cache.n_kv_head} heads of {cache.head_dim} and {cache.head_dim_v}")
         if k.dtype != v.dtype:
             raise TypeError(f"tensor-cuda: kv_append: dtype mismatch {k.dtype} vs {v.dtype} (no implicit promotion)")
-        tok = self._kv_tokens("kv_append", cache, table, pos, seq, k.shape[0])
-        tok.k_stride[:] = [cache.n_kv_head * cache.head_dim, cache.head_dim]
-        tok.v_stride[:] = [cache.n_kv_head * cache.head_dim_v, cache.head_dim_v]
-        self._append(cache, tok, k.dtype, k.ptr, v.ptr, table, pos, seq)
+        self._append("kv_append", cache, k.dtype, k.shape[0], cache.k_strides, cache.v_strides, k.ptr, v.ptr, table, pos, seq)
 
     def kv_append_packed(self, cache, qkv: CudaTensor, table: CudaTensor, pos: CudaTensor,
                          seq: CudaTensor | None = None) -> None:
@@ -802,13 +801,12 @@ class CudaBackend:
         then the cache's K heads, then its V heads (``sdpa_packed``'s layout, with H = Hk)."""
         self._mine("kv_append_packed", qkv)
         n_q = self._packed_heads("kv_append_packed", cache, qkv)
-        tok = self._kv_tokens("kv_append_packed", cache, table, pos, seq, qkv.shape[0])
         width, d = qkv.shape[1], cache.head_dim
-        tok.k_stride[:] = [width, d]
-        tok.v_stride[:] = [width, d]
         eb = F.DTYPE_BYTES[F.DTYPE_CODES[qkv.dtype]]
         k = qkv.ptr + n_q * d * eb
-        self._append(cache, tok, qkv.dtype, k, k + cache.n_kv_head * d * eb, table, pos, seq)
+        strides = F.I64x2(width, d)
+        self._append("kv_append_packed", cache, qkv.dtype, qkv.shape[0], strides, strides, k, k + cache.n_kv_head * d * eb,
+                     table, pos, seq)
 
     @staticmethod
     def _packed_heads(where: str, cache, qkv: CudaTensor) -> int:
@@ -819,12 +817,13 @@ class CudaBackend:
                              f"{cache.head_dim_v}")
         return n_q
 
-    def _append(self, cache, tok, dtype: str, k: int, v: int, table, pos, seq) -> None:
+    def _append(self, where: str, cache, dtype: str, n: int, k_strides, v_strides, k: int, v: int, table, pos, seq) -> None:
+        self._kv_places(where, cache, table, pos, seq, n)
         if dtype not in FLOAT or (cache.dtype != "e4m3" and dtype != cache.dtype):
-            raise TypeError(f"tensor-cuda: kv_append: {dtype} rows into a {cache.dtype} cache (no implicit promotion)")
-        tok.dtype = F.DTYPE_CODES[dtype]
-        F.call("mpc_kv_append", self.device.handle, *cache.args, C.byref(tok), C.c_void_p(k), C.c_void_p(v),
-               C.c_void_p(table.ptr), C.c_void_p(seq.ptr if seq is not None else None), C.c_void_p(pos.ptr), None)
+            raise TypeError(f"tensor-cuda: {where}: {dtype} rows into a {cache.dtype} cache (no implicit promotion)")
+        tok = F.KvTokens(n, table.shape[0], table.shape[1], k_strides, v_strides, F.DTYPE_CODES[dtype], 0)
+        F.call("mpc_kv_append", self.device.handle, *cache.args, C.byref(tok), k, v, table.ptr,
+               None if seq is None else seq.ptr, pos.ptr, None)
 
     @staticmethod
     def _check_out(where: str, out: CudaTensor, shape, dtype: str) -> CudaTensor:
@@ -838,7 +837,7 @@ class CudaBackend:
         """The rows at (seq[t], pos[t]) as dense (k [T, Hk, D], v [T, Hk, Dv]) of ``dtype`` (default: the cache's;
         bf16 for an 8-bit cache), rounded once; zeros where pos < 0. ``out``: the (k, v) to write into."""
         n = pos.shape[0] if pos.shape else 0
-        tok = self._kv_tokens("kv_read", cache, table, pos, seq, n)
+        self._kv_places("kv_read", cache, table, pos, seq, n)
         dtype = dtype or ("bf16" if cache.dtype == "e4m3" else cache.dtype)
         if dtype not in FLOAT:
             raise TypeError(f"tensor-cuda: kv_read: float dtypes only, got {dtype}")
@@ -848,11 +847,9 @@ class CudaBackend:
         else:
             self._mine("kv_read", *out)
             k, v = (self._check_out("kv_read", o, s, dtype) for o, s in zip(out, shapes))
-        tok.k_stride[:] = [shapes[0][1] * shapes[0][2], shapes[0][2]]
-        tok.v_stride[:] = [shapes[1][1] * shapes[1][2], shapes[1][2]]
-        tok.dtype = F.DTYPE_CODES[dtype]
-        F.call("mpc_kv_read", self.device.handle, *cache.args, C.byref(tok), C.c_void_p(k.ptr), C.c_void_p(v.ptr),
-               C.c_void_p(table.ptr), C.c_void_p(seq.ptr if seq is not None else None), C.c_void_p(pos.ptr), None)
+        tok = F.KvTokens(n, table.shape[0], table.shape[1], cache.k_strides, cache.v_strides, F.DTYPE_CODES[dtype], 0)
+        F.call("mpc_kv_read", self.device.handle, *cache.args, C.byref(tok), k.ptr, v.ptr, table.ptr,
+               None if seq is None else seq.ptr, pos.ptr, None)
         return k, v
 
     def sdpa_paged(self, q: CudaTensor, cache, table: CudaTensor, lengths: CudaTensor, scale: float, lse: bool = False,
@@ -880,7 +877,7 @@ class CudaBackend:
         return merged
 
     def _sdpa_paged(self, q: int, dtype: str, q_stride, B: int, H: int, cache, table, lengths, scale, lse, out):
-        tok = self._kv_tokens("sdpa_paged", cache, table, lengths, None, B)
+        self._kv_places("sdpa_paged", cache, table, lengths, None, B)
         if table.shape[0] != B:
             raise ValueError(f"tensor-cuda: sdpa_paged: {B} queries for {table.shape[0]} sequences")
         if dtype not in FLOAT or (cache.dtype != "e4m3" and dtype != cache.dtype):
@@ -896,13 +893,10 @@ class CudaBackend:
             self._check_out("sdpa_paged", o, shape, dtype)
             if z is not None:
                 self._check_out("sdpa_paged", z, (B, H), "f32")
-        desc = F.SdpaPagedDesc()
-        desc.b, desc.h, desc.max_pages = B, H, tok.max_pages
-        desc.q_stride[:] = q_stride
-        desc.o_stride[:] = (H * cache.head_dim_v, cache.head_dim_v)
-        desc.dtype, desc.scale = F.DTYPE_CODES[dtype], scale
-        F.call("mpc_sdpa_paged", self.device.handle, *cache.args, C.byref(desc), C.c_void_p(q), C.c_void_p(table.ptr),
-               C.c_void_p(lengths.ptr), C.c_void_p(o.ptr), C.c_void_p(z.ptr if z is not None else None), None, 0, None)
+        desc = F.SdpaPagedDesc(B, H, table.shape[1], F.I64x2(*q_stride),
+                               F.I64x2(H * cache.head_dim_v, cache.head_dim_v), F.DTYPE_CODES[dtype], scale)
+        F.call("mpc_sdpa_paged", self.device.handle, *cache.args, C.byref(desc), q, table.ptr, lengths.ptr, o.ptr,
+               None if z is None else z.ptr, None, 0, None)
         return (o, z) if lse else o
 
     def sample(self, logits: CudaTensor, u: CudaTensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -920,8 +914,7 @@ class CudaBackend:
         if logits.dtype not in FLOAT:
             raise TypeError(f"tensor-cuda: sample: float logits only, got {logits.dtype}")
         B, V = logits.shape
-        desc = F.SampleDesc()
-        desc.rows, desc.vocab, desc.row_stride, desc.dtype = B, V, V, F.DTYPE_CODES[logits.dtype]
+        desc = F.SampleDesc(B, V, V, F.DTYPE_CODES[logits.dtype])
         per_row = []
         for name, x, dt in (("u", u, "f32"), ("temperature", temperature, "f32"), ("top_k", top_k, "i32"),
                             ("top_p", top_p, "f32"), ("min_p", min_p, "f32")):
@@ -930,7 +923,7 @@ class CudaBackend:
                 if x.shape != (B,) or x.dtype != dt:
                     raise TypeError(f"tensor-cuda: sample: {name} is {dt} [{B}], got {x.dtype} "
                                     f"[{','.join(map(str, x.shape))}]")
-                per_row.append(C.c_void_p(x.ptr))
+                per_row.append(x.ptr)
             elif name == "u":
                 raise TypeError("tensor-cuda: sample: u is an f32 array, one uniform number per row")
             else:
@@ -945,8 +938,8 @@ class CudaBackend:
             self._mine("sample", *outs)
             for o, dt in zip(outs, ("i32", "f32", "i32")):
                 self._check_out("sample", o, (B,), dt)
-        F.call("mpc_sample", self.device.handle, C.byref(desc), C.c_void_p(logits.ptr), *per_row,
-               *(C.c_void_p(o.ptr) for o in outs), *([None] * (3 - len(outs))), None)
+        F.call("mpc_sample", self.device.handle, C.byref(desc), logits.ptr, *per_row, *(o.ptr for o in outs),
+               *([None] * (3 - len(outs))), None)
         return tuple(outs) if details else outs[0]
 
     def layerNorm(self, x: CudaTensor, weight: CudaTensor | None, bias: CudaTensor | None, eps: float = 1e-5):

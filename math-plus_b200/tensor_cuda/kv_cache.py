@@ -51,6 +51,9 @@ class PagedKVCache:
             raise ValueError("tensor-cuda: PagedKVCache: pools are four addresses (K, V, K scales, V scales)")
         #: (desc, K pages, V pages, K scales, V scales) as every call of the C ABI takes them
         self.args = (C.byref(self.desc), *(C.c_void_p(p) for p in pools))
+        #: element strides (token, head) of dense rows [T, Hk, D]
+        self.k_strides = F.I64x2(self.n_kv_head * self.head_dim, self.head_dim)
+        self.v_strides = F.I64x2(self.n_kv_head * self.head_dim_v, self.head_dim_v)
         self.disposed = False
 
     def dispose(self) -> None:
