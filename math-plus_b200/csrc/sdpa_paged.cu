@@ -167,8 +167,12 @@ __device__ __forceinline__ void empty_rows(const Params &p) {
   }
 }
 
-__device__ __forceinline__ void put(const Params &p, int b, int h, int e, float v, float sum, float top, float otop) {
-  store_f32(p.out, p.dt, b * p.os[0] + h * p.os[1] + e, sum != 0.0f ? v * exp2f(otop - top) / sum : 0.0f);
+// Column e of (sequence, head), and with it the row's log-sum-exp: f = 2^(otop - top) / sum.
+__device__ __forceinline__ float factor_of(float sum, float top, float otop) {
+  return sum != 0.0f ? exp2f(otop - top) / sum : 0.0f;
+}
+__device__ __forceinline__ void put(const Params &p, int b, int h, int e, float v, float f, float sum, float top) {
+  store_f32(p.out, p.dt, b * p.os[0] + h * p.os[1] + e, sum != 0.0f ? v * f : 0.0f);
   if (p.lse && e == 0) p.lse[(long long)b * p.H + h] = sum != 0.0f ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
 }
 
@@ -201,7 +205,7 @@ __device__ __forceinline__ void finish(const Params &p, const Item &it, int t0, 
     float top, otop, sum, v;
     combine<SRC>(so, sml, q, e, v, sum, top, otop);
     if (whole) {
-      put(p, it.b, h0 + q, e, v, sum, top, otop);
+      put(p, it.b, h0 + q, e, v, factor_of(sum, top, otop), sum, top);
     } else {
       float *ws = slot(p, gw, t0 == 0, q);
       ws[4 + e] = v;
@@ -236,54 +240,85 @@ __device__ __forceinline__ bool last_part(const Params &p, const Deal &all, cons
   return true;
 }
 
-// One warp joins query q of an item, eight parts' loads in flight: every lane reads a part's header and four or
-// eight columns of its O.
+// One warp joins query q of an item: lanes hold the parts' headers and weights, 32 at a time, then each lane columns
+// 4 lane ..+3 (WIDE: + 128 too) of their O, eight parts' loads in flight. (A single warp's instructions bound this,
+// so a part costs few.) Places that a lane has no column or a round no part for repeat another with weight 0.
+template <bool WIDE>
 __device__ __forceinline__ void join(const Params &p, const Deal &all, const Join &j, int q) {
+  constexpr int E = WIDE ? 2 : 1;
   const int lane = threadIdx.x & 31;
   const int kvh = j.it.head / p.qt, h = kvh * p.group + (j.it.head % p.qt) * p.gt + q;
-  const bool in0 = 4 * lane < p.dv, in1 = 4 * lane + 128 < p.dv;
+  const int row = slot_floats(p.dv) / 4, step = 2 * p.gt * row;  // float4s from a place to the next, of a warp to the next
+  const float4 *const places = reinterpret_cast<const float4 *>(p.ws) + (long long)j.first * step + q * row;
+  const int start = p.gt * row;  // the first part is in its warp's second place
+  int col[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) col[e] = 128 * e + 4 * lane < p.dv ? 1 + 32 * e + lane : 1;
   float top = -INFINITY, otop = -INFINITY, sum = 0.0f;
-  float4 v[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-  for (int w = j.first; w <= j.last;) {
-    float4 x[8], z[8][2];
+  float4 v[E];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      x[k] = make_float4(-INFINITY, -INFINITY, 0, 0);
-      z[k][0] = z[k][1] = make_float4(0, 0, 0, 0);
-      if (w <= j.last) {
-        const float4 *y = reinterpret_cast<const float4 *>(slot(p, w, w == j.first, q));
-        x[k] = __ldcg(y);
-        if (in0) z[k][0] = __ldcg(y + 1 + lane);
-        if (in1) z[k][1] = __ldcg(y + 33 + lane);
-        w += w % kWarps == 0 && meets(all, j.it, w / kWarps) ? kWarps : 1;
-      }
+  for (int e = 0; e < E; ++e) v[e] = make_float4(0, 0, 0, 0);
+  // The parts: the first block's warps from j.first on (or one, where they met), one of every block inside the
+  // item, the last block's warps up to j.last (or one).
+  const int b0 = j.first / kWarps, b1 = j.last / kWarps;
+  const int n0 = meets(all, j.it, b0) ? 1 : min((b0 + 1) * kWarps, j.last + 1) - j.first;
+  const int n1 = b1 > b0 ? n0 + b1 - b0 - 1 : n0;
+  const int parts = b1 == b0 ? n0 : n1 + (meets(all, j.it, b1) ? 1 : j.last - b1 * kWarps + 1);
+  auto warp_of = [&](int i) {  // less j.first
+    return i < n0 ? i : (i < n1 ? (b0 + 1 + i - n0) * kWarps : b1 * kWarps + i - n1) - j.first;
+  };
+  for (int base = 0; base < parts; base += 32) {
+    const int mine = warp_of(min(base + lane, parts - 1));
+    float4 x = make_float4(-INFINITY, -INFINITY, 0, 0);
+    if (base + lane < parts) x = __ldcg(places + (long long)mine * step + (mine ? 0 : start));
+    float up = x.x, oup = x.y;
+#pragma unroll
+    for (int k = 16; k; k >>= 1) {
+      up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, k));
+      oup = fmaxf(oup, __shfl_xor_sync(0xffffffffu, oup, k));
     }
-    float up = top, oup = otop;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) up = fmaxf(up, x[k].x), oup = fmaxf(oup, x[k].y);
-    sum *= guard_exp2(top, up);
+    up = fmaxf(up, top), oup = fmaxf(oup, otop);
     const float keep = guard_exp2(otop, oup);
+    float l = x.z * guard_exp2(x.x, up);
+    const float f = guard_exp2(x.y, oup);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) v[e].x *= keep, v[e].y *= keep, v[e].z *= keep, v[e].w *= keep;
+    for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    sum = fmaf(sum, guard_exp2(top, up), l);
     top = up, otop = oup;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      sum = fmaf(x[k].z, guard_exp2(x[k].x, top), sum);
-      const float f = guard_exp2(x[k].y, otop);
+    for (int e = 0; e < E; ++e) v[e].x *= keep, v[e].y *= keep, v[e].z *= keep, v[e].w *= keep;
+    unsigned left = __ballot_sync(0xffffffffu, f != 0.0f);
+    while (left) {
+      float4 z[8][E];
+      float wt[8];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        v[e].x = fmaf(z[k][e].x, f, v[e].x), v[e].y = fmaf(z[k][e].y, f, v[e].y);
-        v[e].z = fmaf(z[k][e].z, f, v[e].z), v[e].w = fmaf(z[k][e].w, f, v[e].w);
+      for (int k = 0; k < 8; ++k) {
+        const int i = left ? __ffs(left) - 1 : 0;
+        wt[k] = __shfl_sync(0xffffffffu, f, i);
+        if (!left) wt[k] = 0.0f;
+        const int at = __shfl_sync(0xffffffffu, mine, i);
+        const float4 *y = places + (long long)at * step + (at ? 0 : start);
+        left &= left - 1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[k][e] = __ldcg(y + col[e]);
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          v[e].x = fmaf(z[k][e].x, wt[k], v[e].x), v[e].y = fmaf(z[k][e].y, wt[k], v[e].y);
+          v[e].z = fmaf(z[k][e].z, wt[k], v[e].z), v[e].w = fmaf(z[k][e].w, wt[k], v[e].w);
+        }
     }
   }
+  const float f = factor_of(sum, top, otop);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
+  for (int e = 0; e < E; ++e) {
     const float y[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 4; ++k) {
       const int at = 128 * e + 4 * lane + k;
-      if (at < p.dv) put(p, j.it.b, h, at, y[k], sum, top, otop);
+      if (at < p.dv) put(p, j.it.b, h, at, k < 2 ? (k ? y[1] : y[0]) : (k == 2 ? y[2] : y[3]), f, sum, top);
     }
   }
 }
@@ -363,9 +398,13 @@ __device__ __forceinline__ void walk(const Params &p, float (*so)[GT][PITCH], fl
   }
   empty_rows(p);
   __syncthreads();
-  for (int i = warp; i < n_joins * GT; i += kWarps) {
-    const Join j = joins[i / GT];
-    if (i % GT < p.group - (j.it.head % p.qt) * GT) join(p, all, j, i % GT);
+  const int queries = min(GT, p.group);
+  for (int i = warp; i < n_joins * queries; i += kWarps) {
+    const Join j = joins[i / queries];
+    const int q = i % queries;
+    if (q >= p.group - (j.it.head % p.qt) * GT) continue;
+    if (p.dv > 128) join<true>(p, all, j, q);
+    else join<false>(p, all, j, q);
   }
 }
 
