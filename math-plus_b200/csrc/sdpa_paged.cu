@@ -27,9 +27,9 @@ namespace paged {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 4;  // resident on an SM, at most
-// Measured (GPU time; 0, 4, 8, 12, 24 tiles an item): 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 35, 28, 27,
-// 28, 33 us; 32 sequences of 500..8191 keys, 8 heads of 128, f16: 109, 100, 98, 98, 99 us; 2 of ~115k keys in 8 bits:
-// 103, 95, 91, 90, 92 us.
+// Measured (3, 5, 8, 12 tiles an item): 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 23.5, 24.3, 25.2, 26.7 us; 32
+// sequences of 500..8191 keys, 8 heads of 128, f16: 100.8, 100.1, 98.5, 98.5 us; 2 of ~115k keys in 8 bits: 112, 111, 107,
+// 100 us. (0, before the join had its present form: 35, 109 and 103 against 27, 98 and 91 us.)
 constexpr int kItemCost = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -432,23 +432,39 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
       for (int e = 0; e < NI * 8; ++e) o[q][e] = 0.0f;
     }
     const unsigned end = (unsigned)min((long long)length_of(p, b), (long long)t1 * p.tile);  // lengths are below 2^31
-    for (unsigned k0 = (unsigned)t0 * (unsigned)p.tile; k0 < end; k0 += 4) {
+    // The row of this group's key, k0 + lane / 8; -1: none (behind the end, or a page outside the cache).
+    auto row_at = [&](unsigned k0) -> long long {
       const unsigned key = k0 + (lane >> 3);
-      long long row = -1;
-      if (key < end) {
-        const unsigned col = p.page_of(key);
-        const int pg = p.table[(long long)b * p.max_pages + col];
-        if (pg >= 0 && pg < p.n_pages) row = ((long long)pg * p.hk + kvh) * p.page_size + (key - col * (unsigned)p.page_size);
-        else if ((lane & 7) == 0) report_bad_page(p.err, kBadAttend, b);
-      }
+      if (key >= end) return -1;
+      const unsigned col = p.page_of(key);
+      const int pg = p.table[(long long)b * p.max_pages + col];
+      if (pg >= 0 && pg < p.n_pages) return ((long long)pg * p.hk + kvh) * p.page_size + (key - col * (unsigned)p.page_size);
+      if ((lane & 7) == 0) report_bad_page(p.err, kBadAttend, b);
+      return -1;
+    };
+    // Where the registers allow, a key's V and the next step's row are under way with its K.
+    constexpr bool AHEAD = VEC && NI * GT <= 4;
+    unsigned k0 = (unsigned)t0 * (unsigned)p.tile;
+    long long row = row_at(k0);
+    for (; k0 < end; k0 += 4) {
       float s[GT], x[8];
+      Raw8 k_raw[AHEAD ? NI : 1], v_raw[AHEAD ? NI : 1];
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (row >= 0 && i * 64 + j8 < p.d) load_raw8(p.kp, p.dt_pages, row * p.d + i * 64 + j8, k_raw[i]);
+          if (row >= 0 && i * 64 + j8 < p.dv) load_raw8(p.vp, p.dt_pages, row * p.dv + i * 64 + j8, v_raw[i]);
+        }
+      }
+      const long long next = row_at(k0 + 4);
 #pragma unroll
       for (int q = 0; q < GT; ++q) s[q] = 0.0f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int at = i * 64 + j8;
         if (row >= 0 && at < p.d) {
-          load8<VEC>(p.kp, p.dt_pages, row * p.d + at, p.d - at, x);
+          if constexpr (AHEAD) widen8(k_raw[i], p.dt_pages, x);
+          else load8<VEC>(p.kp, p.dt_pages, row * p.d + at, p.d - at, x);
 #pragma unroll
           for (int q = 0; q < GT; ++q)
 #pragma unroll
@@ -459,33 +475,36 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
       for (int q = 0; q < GT; ++q)
 #pragma unroll
         for (int k = 4; k; k >>= 1) s[q] += __shfl_xor_sync(0xffffffffu, s[q], k);
-      if (row < 0) continue;
-      const float f = p.scale_log2 * (p.dt_pages == MPC_E4M3 ? scale_value(p.ks[row]) : 1.0f);
+      if (row >= 0) {
+        const float f = p.scale_log2 * (p.dt_pages == MPC_E4M3 ? scale_value(p.ks[row]) : 1.0f);
 #pragma unroll
-      for (int q = 0; q < GT; ++q) {
-        s[q] *= f;
-        const float top = fmaxf(m[q], s[q]);
-        const float keep = guard_exp2(m[q], top);
-        s[q] = guard_exp2(s[q], top);
-        m[q] = top;
-        l[q] = fmaf(l[q], keep, s[q]);
+        for (int q = 0; q < GT; ++q) {
+          s[q] *= f;
+          const float top = fmaxf(m[q], s[q]);
+          const float keep = guard_exp2(m[q], top);
+          s[q] = guard_exp2(s[q], top);
+          m[q] = top;
+          l[q] = fmaf(l[q], keep, s[q]);
 #pragma unroll
-        for (int e = 0; e < NI * 8; ++e) o[q][e] *= keep;
-      }
-      const float fv = p.dt_pages == MPC_E4M3 ? scale_value(p.vs[row]) : 1.0f;
+          for (int e = 0; e < NI * 8; ++e) o[q][e] *= keep;
+        }
+        const float fv = p.dt_pages == MPC_E4M3 ? scale_value(p.vs[row]) : 1.0f;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int at = i * 64 + j8;
-        if (at < p.dv) {
-          load8<VEC>(p.vp, p.dt_pages, row * p.dv + at, p.dv - at, x);
+        for (int i = 0; i < NI; ++i) {
+          const int at = i * 64 + j8;
+          if (at < p.dv) {
+            if constexpr (AHEAD) widen8(v_raw[i], p.dt_pages, x);
+            else load8<VEC>(p.vp, p.dt_pages, row * p.dv + at, p.dv - at, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = x[e] * fv;
+            for (int e = 0; e < 8; ++e) {
+              const float v = x[e] * fv;
 #pragma unroll
-            for (int q = 0; q < GT; ++q) o[q][i * 8 + e] = fmaf(s[q], v, o[q][i * 8 + e]);
+              for (int q = 0; q < GT; ++q) o[q][i * 8 + e] = fmaf(s[q], v, o[q][i * 8 + e]);
+            }
           }
         }
       }
+      row = next;
     }
     // The 4 groups of the warp meet by shuffles.
 #pragma unroll
@@ -616,7 +635,7 @@ __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND
 // DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value; LO: weights as two
 // numbers. TPI tiles of 16
 // keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks per SM as the registers
-// allow; over 8-bit rows of 128 two blocks of 32 keys a warp (91 us at 2 x ~115k keys) beat three or four of 16 (100 us).
+// allow; over 8-bit rows of 128 two blocks of 32 keys a warp (94 us at 2 x ~115k keys, the join left out) beat three of 16 (100 us).
 template <int KIND, int DP>
 constexpr int tiles_at_once() { return DP == 64 || (DP == 128 && KIND == kE4M3) ? 2 : 1; }
 constexpr int blocks_per_sm(bool e4m3, int dp, int heads) { return dp == 256 || heads == 16 || (dp == 128 && e4m3) ? 2 : 3; }
