@@ -16,6 +16,10 @@
 // Both directions are bound by HBM. A row of up to 256 values is one group of 8, 16 or 32 lanes,
 // 8 values (16 bytes of a 16-bit type) per lane, so that the row's maximum is a few shuffles and the
 // row is read once; a group keeps its token's place over the heads it walks.
+//
+// Measured (GPU time of a replayed call): 32768 tokens of 8 heads of 128, bf16 to 8 bits, 38.3 us (5.1 TB/s); 49152
+// such tokens from 8 bits to bf16 54.4 us (5.6 TB/s), of a measured copy rate of 6.55; 8 tokens of 12 heads of 64, bf16,
+// 2.5 us, where a chain of latencies bounds it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -24,7 +24,9 @@
 //
 // A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy. A few rows are bound by latency (cluster
 // barriers and remote reads), many by the instructions per token of the passes, the f64 exponentials (10 double
-// operations each) of the rows without top_k above all.
+// operations each) of the rows without top_k above all. Measured (GPU time of a replayed call): 4 rows of 50257 bf16 with
+// mixed settings 15.8 us (15 to 58 by the numbers drawn); 256 rows of 131071 f32 with mixed settings 215 us; such rows
+// alike, greedy 49, top_k 50 100, no filter 139, top_p 0.9 350 us; 128 MB at 6.55 TB/s are 20.5 us.
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
