@@ -261,7 +261,7 @@ int mpc_device_create(int ordinal, unsigned flags, mpc_device **out) {
   if ((e = cudaStreamCreateWithFlags(&dev->stream, cudaStreamNonBlocking)) != cudaSuccess ||
       (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess || (e = cudaMemset(dev->d_err, 0, 256)) != cudaSuccess ||
       (e = cudaMalloc(&dev->d_counters, kCounterBytes)) != cudaSuccess ||
-      (e = cudaMemset(dev->d_counters, 0, kCounterBytes)) != cudaSuccess) {
+      (e = cudaMemsetAsync(dev->d_counters, 0, kCounterBytes, dev->stream)) != cudaSuccess) {
     rc = cuda_fail(nullptr, e, "mpc_device_create");
     if (dev->d_err) cudaFree(dev->d_err);
     if (dev->d_counters) cudaFree(dev->d_counters);
