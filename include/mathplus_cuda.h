@@ -347,7 +347,8 @@ int mpc_kv_read(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, 
  * [b, h, dv] have element strides (sequence, head) and a contiguous last axis; their dtype is the cache's,
  * or any float type over MPC_E4M3. LSE (optional, f32 [b, h]) is the natural-log normaliser. The work is
  * split along the cache by the lengths found on the device; the partial results live in the workspace
- * until the block that completes an item joins them. A length that is negative or beyond max_pages * page_size, or a
+ * until the block that completes an item joins them. An infinity or a NaN in a row within the length makes the
+ * values that depend on it NaN or infinite, which of the two is not defined. A length that is negative or beyond max_pages * page_size, or a
  * page outside the cache, is cut off or left out, and the next synchronisation returns MPC_ERR_INVALID. */
 typedef struct {
   int64_t b, h, max_pages;

@@ -5,7 +5,8 @@
 // upper reference of s' (the running maximum). Every K/V row is read once and used for the query
 // heads that share it, so the cache's bytes bound the time and the work is split along the cache:
 //
-// Split. An item is (sequence, K/V head, tile of its query heads); its keys are cut into tiles (16 or 32). The
+// Split. An item is (sequence, K/V head, tile of its query heads); its keys are cut into tiles (16 or 32; more
+// where a table could hold 2^30 of them). The
 // tiles of all items, in order, with kItemCost more for every item (an item's start and end take about
 // as long as that many tiles), are dealt to the warps in equal runs: warp i of n takes units [T i / n,
 // T (i + 1) / n). The runs are found from the lengths on the device, so ragged batches and a single long
@@ -639,9 +640,9 @@ __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND
 }
 
 // DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value; LO: weights as two
-// numbers. TPI tiles of 16
-// keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks per SM as the registers
-// allow; over 8-bit rows of 128 two blocks of 32 keys a warp (94 us at 2 x ~115k keys, the join left out) beat three of 16 (100 us).
+// numbers. TPI tiles of 16 keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks
+// per SM as the registers allow; over 8-bit rows of 128 two blocks of 32 keys a warp (94 us at 2 x ~115k keys, the join
+// left out) beat three of 16 (100 us).
 template <int KIND, int DP>
 constexpr int tiles_at_once() { return DP == 64 || (DP == 128 && KIND == kE4M3) ? 2 : 1; }
 constexpr int blocks_per_sm(bool e4m3, int dp, int heads) { return dp == 256 || heads == 16 || (dp == 128 && e4m3) ? 2 : 3; }

@@ -282,8 +282,10 @@ class GPT2Session:
     def generate(self, prompts, max_new: int, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> list:
         """Continues every prompt (a list of token lists, one per sequence) by ``max_new`` tokens drawn with
         ``CudaBackend.sample`` from the uniform numbers u [n_seq, max_new] (none needed with temperature 0: the
-        best token). Returns the new tokens. The session goes on from there."""
-        be = self.model.backend
+        best token). Returns the new tokens. The session goes on from there; the last token drawn has not been
+        fed yet, so the next ids begin with it. Pages for all of it are taken first: when the pool or the context
+        is too small nothing has changed."""
+        be, n_ctx = self.model.backend, self.model.cfg.n_ctx
         if len(prompts) != self.n_seq or not all(len(p) for p in prompts):
             raise ValueError(f"GPT2Session: {len(prompts)} prompts for {self.n_seq} sequences, none of them empty")
         if u is None:
@@ -293,6 +295,11 @@ class GPT2Session:
         u = np.asarray(u, np.float32)
         if u.shape != (self.n_seq, max_new):
             raise ValueError(f"GPT2Session: u [{','.join(map(str, u.shape))}] for {self.n_seq} sequences of {max_new} tokens")
+        if max_new:
+            after = [s + len(p) + max_new - 1 for s, p in zip(self.lengths, prompts)]
+            if max(after) > n_ctx:
+                raise ValueError(f"GPT2Session: {max(after)} tokens are more than the context ({n_ctx})")
+            self.table.reserve(after)
         longest = max(len(p) for p in prompts)
         ids = np.zeros((self.n_seq, longest), np.int32)
         for row, p in zip(ids, prompts):

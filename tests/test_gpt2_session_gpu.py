@@ -128,3 +128,21 @@ def test_sessions_refuse(setup):
     with pytest.raises(ValueError, match="ids"):
         s.step(np.zeros((2, 3), np.int32))
     s.dispose()
+
+
+def test_generate_takes_all_or_nothing(setup):
+    """A stretch that the pool or the context cannot hold to its end changes nothing; the longest that fits runs."""
+    be, cfg, w, model = setup
+    s = model.session(2, n_pages=4, page_size=16)
+    with pytest.raises(MemoryError, match="free"):
+        s.generate([[1, 2, 3], [4]], 31, temperature=0.0)  # 33 and 31 tokens: 3 + 2 pages
+    assert s.lengths == [0, 0] and s.table.free_pages == 4
+    got = s.generate([[1, 2, 3], [4]], 30, temperature=0.0)  # 32 and 30
+    assert s.lengths == [32, 30] and [len(g) for g in got] == [30, 30] and s.table.free_pages == 0
+    s.dispose()
+    s = model.session(1)
+    with pytest.raises(ValueError, match="context"):
+        s.generate([[1] * 200], 58, temperature=0.0)  # 257 of 256
+    assert s.lengths == [0]
+    assert len(s.generate([[1] * 200], 57, temperature=0.0)[0]) == 57 and s.lengths == [256]
+    s.dispose()
