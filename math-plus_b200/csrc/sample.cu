@@ -292,7 +292,7 @@ __device__ __forceinline__ void count_if(uint32_t counts0, float at, float end) 
 // The histogram's bins: by value below the largest logit (the last bin is not used: what lies deeper is not
 // counted), or by the keys of an interval.
 struct Bins {
-  float top, scale;  // by value: bins of T / 128
+  float top, scale;  // by value: bins of T / 256
   uint32_t lo, hi;   // by key: the interval; lo 0: by value
   int shift;
   // 2^23 + the distance below top in bins: its bits are the bin's number, and NaN and infinities compare as deep.
