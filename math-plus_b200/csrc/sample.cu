@@ -14,8 +14,8 @@
 //      compared with every other. An estimate that was off moves; a bin of more tokens is cut again, by the bits
 //      of its logits.
 //   4. Where the gathered tokens are the whole kept set (a small top_k, a narrow top_p) the draw is among them.
-//      Else every warp has the kept weight of its stretch of the row, and the one that the draw falls into
-//      walks its stretch.
+//      Else every warp has the kept weight of its stretch of the row, and the block with the one that the draw falls
+//      into goes through that stretch again, a piece per thread.
 // Rows are read again by each step, from L1 or L2; HBM is read once.
 //
 // Weights w = exp((l - max) / T) in f64 are held as integers of 2^-shift (shift = 62 - log2 of the row's length, at
@@ -828,69 +828,93 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   __syncthreads();
   const u64 tie_w = key ? wt.whole(logit_of(key)) : 0;
   if (key && !passes(at_key)) ties = 0;
-  // Each warp walks the stretches up to its own, lane by lane of 32.
-  u64 total = 0, before = 0, mine = 0;
-  unsigned kept = 0, tie_before = 0, tie_at = 0;
-  const int self = rank * kWarps + warp;
-  for (int i0 = 0; i0 < C * kWarps; i0 += 32) {
+  // Every warp walks the stretches, lane by lane of 32, and finds the one that the draw falls into.
+  constexpr int kRounds = (C * kWarps + 31) / 32;
+  u64 total = 0, from[kRounds], own[kRounds];
+  unsigned kept = 0, tie_at = 0, ties_from[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
     Sums s{0, 0, 0};
-    if (i0 + lane < C * kWarps) s = sm.every[i0 + lane];
-    const unsigned tie_incl = tie_at + warp_incl(s.ties), tie_excl = tie_incl - s.ties;
-    const unsigned take = min(ties, tie_incl) - min(ties, tie_excl);
-    const u64 w = s.w + take * tie_w, incl = total + warp_incl(w);
+    if (32 * i + lane < C * kWarps) s = sm.every[32 * i + lane];
+    const unsigned tie_incl = tie_at + warp_incl(s.ties);
+    ties_from[i] = tie_incl - s.ties;
+    const unsigned take = min(ties, tie_incl) - min(ties, ties_from[i]);
+    own[i] = s.w + take * tie_w;
+    const u64 incl = total + warp_incl(own[i]);
+    from[i] = incl - own[i];
     const unsigned n = warp_incl(s.n + take);
-    if (i0 <= self && self < i0 + 32) {
-      mine = __shfl_sync(0xffffffffu, w, self - i0);
-      before = __shfl_sync(0xffffffffu, incl, self - i0) - mine;
-      tie_before = __shfl_sync(0xffffffffu, tie_excl, self - i0);
-    }
     total = __shfl_sync(0xffffffffu, incl, 31);
     kept += __shfl_sync(0xffffffffu, n, 31);
     tie_at = __shfl_sync(0xffffffffu, tie_incl, 31);
   }
   if (rank == 0 && threadIdx.x == 0 && p.kept) p.kept[row] = (int32_t)kept;
   const u64 d = draw_of(total);
-  if (before <= d && d < before + mine) {
-    constexpr int VE = Reader<DT>::VE;
-    u64 at = before;
-    unsigned tie = tie_before;
-    for (int v = v0; v < v1; v += 32) {
+  int stretch = 0;
+  u64 before = 0;
+  unsigned tie_before = 0;
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const unsigned hit = __ballot_sync(0xffffffffu, from[i] <= d && d < from[i] + own[i]);
+    if (!hit) continue;
+    stretch = 32 * i + __ffs(hit) - 1;
+    before = __shfl_sync(0xffffffffu, from[i], __ffs(hit) - 1);
+    tie_before = __shfl_sync(0xffffffffu, ties_from[i], __ffs(hit) - 1);
+  }
+  if (stretch / kWarps == rank) {
+    // The block takes the stretch in pieces, one per thread, then the warp of the piece with the draw takes that, one
+    // token per lane. (One warp alone on the stretch waited for its exponentials longer than the rest of the row's work
+    // took: 57 000 of 97 000 cycles at 131071 tokens.)
+    auto weight_of = [&](float f) -> u64 {  // of a token that is not a tie
+      if (!(f >= low) || !(f >= sure || passes(f))) return 0;
+      return wt.whole(f);
+    };
+    const int s0 = min(c1, rank * per_cta + stretch % kWarps * per_warp), s1 = min(c1, s0 + per_warp);
+    const int piece = (s1 - s0 + kThreads - 1) / kThreads;
+    const int p0 = min(s1, s0 + (int)threadIdx.x * piece), p1 = min(s1, p0 + piece);
+    u64 w = 0, all;
+    unsigned eq = 0, all_eq;
+    for (int v = p0; v < p1; ++v) {
+      constexpr int VE = Reader<DT>::VE;
       float f[VE];
-#pragma unroll
-      for (int k = 0; k < VE; ++k) f[k] = -INFINITY;
-      if (v + lane < v1) rd.load(v + lane, f);
-      unsigned eq = 0;
-#pragma unroll
-      for (int k = 0; k < VE; ++k) eq += f[k] == at_key;
-      const unsigned eq_incl = warp_incl(eq);
-      unsigned my_tie = tie + eq_incl - eq;
-      u64 q[VE], part = 0;
-#pragma unroll
-      for (int k = 0; k < VE; ++k) {
-        q[k] = 0;
-        if (!(f[k] >= low)) continue;
-        if (f[k] == at_key) {
-          if (my_tie++ < ties) q[k] = tie_w;
-        } else if (passes(f[k])) {
-          q[k] = wt.whole(f[k]);
-        }
-        part += q[k];
-      }
-      const u64 incl = at + warp_incl(part);
-      u64 upto = incl - part;
-      if (upto <= d && d < incl) {
+      rd.load(v, f);
+      if (wt.plain) {
 #pragma unroll
         for (int k = 0; k < VE; ++k) {
-          if (upto <= d && d < upto + q[k]) {
-            p.token[row] = rd.index(v + lane) + k;
-            if (p.prob) p.prob[row] = (float)(wt.weight(f[k]) / ((double)total * wt.unit));
-          }
-          upto += q[k];
+          const u64 x = wt.whole_any(f[k]);
+          if (f[k] == at_key) ++eq;
+          else if (f[k] >= low && (f[k] >= sure || passes(f[k]))) w += x;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+          if (f[k] == at_key) ++eq;
+          else w += weight_of(f[k]);
         }
       }
-      at = __shfl_sync(0xffffffffu, incl, 31);
-      if (at > d) break;
-      tie += __shfl_sync(0xffffffffu, eq_incl, 31);
+    }
+    unsigned tie = tie_before + block_incl(eq, sm.warp_n, &all_eq) - eq;
+    u64 at = before + block_incl(w, sm.scratch, &all) - w + (min(ties, tie) - min(ties, tie_before)) * tie_w;
+    w += (min(ties, tie + eq) - min(ties, tie)) * tie_w;
+    const unsigned hit = __ballot_sync(0xffffffffu, at <= d && d < at + w);
+    if (hit) {
+      const int owner = __ffs(hit) - 1;
+      at = __shfl_sync(0xffffffffu, at, owner), tie = __shfl_sync(0xffffffffu, tie, owner);
+      const int end = min(p.vocab, rd.index(__shfl_sync(0xffffffffu, p1, owner)));
+      for (int i = max(0, rd.index(__shfl_sync(0xffffffffu, p0, owner))); i < end; i += 32) {
+        const float f = i + lane < end ? rd.one(i + lane) : -INFINITY;
+        const unsigned ties_in = __ballot_sync(0xffffffffu, f == at_key);
+        u64 q = 0;
+        if (f == at_key) q = tie + __popc(ties_in & ((1u << lane) - 1)) < ties ? tie_w : 0;
+        else q = weight_of(f);
+        const u64 incl = at + warp_incl(q);
+        if (incl - q <= d && d < incl) {
+          p.token[row] = i + lane;
+          if (p.prob) p.prob[row] = (float)(wt.weight(f) / ((double)total * wt.unit));
+        }
+        at = __shfl_sync(0xffffffffu, incl, 31);
+        if (at > d) break;
+        tie += __popc(ties_in);
+      }
     }
   }
   cl.sync();
