@@ -599,17 +599,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         const float g_top = quick ? 0.0f : wt.top, g_scale = quick ? 1.0f : bins.scale, g_bias = quick ? 0.0f : 8388608.0f;
         const float a = quick ? -INFINITY : g_bias + (float)b0, z = quick ? -logit_of(bound) : g_bias + (float)b1;
         rd.batches(v0, v1, [&](const float(&f)[16], int v) {
+          auto at = [&](int k) { return fmaf(g_top - f[k], g_scale, g_bias); };
+          float least = INFINITY;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) least = fminf(least, at(k));
+          if (!__any_sync(0xffffffffu, least <= z)) return;
           unsigned up = 0, in = 0;  // of the 16: those above the window, those in it
           bool doubt = false;       // whether one of those above passes min_p takes its weight to tell
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float x = fmaf(g_top - f[k], g_scale, g_bias);
+            const float x = at(k);
             const bool over = need && x < a;
             up |= over ? 1u << k : 0u;
             in |= x <= z && !(x < a) ? 1u << k : 0u;
             doubt |= over && f[k] >= far && !(f[k] >= sure);
           }
-          if (!__any_sync(0xffffffffu, up | in)) return;
           // The rare tokens are read again, one at a time: a branch for each of the 16 is code that the first warps wait for.
           auto next = [&](unsigned &set) {
             const int k = __ffs(set) - 1;
@@ -629,10 +633,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
           } else if (need && wt.plain && !doubt) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const u64 w = up >> k & 1 ? wt.whole_any(f[k]) : 0;
-              const bool pass = (up >> k & 1) && f[k] >= sure;
-              add_up += w;
-              s.w += pass ? w : 0, s.n += pass;
+              // without a branch, so that the exponentials overlap
+              const unsigned over = up >> k & 1, pass = over & (unsigned)(f[k] >= sure);
+              const u64 w = wt.whole_any(f[k]);
+              add_up += w & (0 - (u64)over);
+              s.w += w & (0 - (u64)pass), s.n += pass;
             }
           } else {
             while (up) note(rd.one(next(up)));
