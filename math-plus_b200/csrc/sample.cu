@@ -25,8 +25,9 @@
 // A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy. A few rows are bound by latency (cluster
 // barriers and remote reads), many by the instructions per token of the passes, the f64 exponentials (10 double
 // operations each) of the rows without top_k above all. Measured (GPU time of a replayed call): 4 rows of 50257 bf16 with
-// mixed settings 15.8 us (15 to 58 by the numbers drawn); 256 rows of 131071 f32 with mixed settings 215 us; such rows
-// alike, greedy 49, top_k 50 100, no filter 139, top_p 0.9 350 us; 128 MB at 6.55 TB/s are 20.5 us.
+// mixed settings 14.8 us (alike: greedy 6, top_k 50 15, top_p 0.9 26, top_k 1000 with top_p and min_p 45); 256 rows of
+// 131071 f32 with mixed settings 174 us (greedy 57, top_k 50 101, no filter 104, top_p 0.9 267); 134 MB at 6.55 TB/s
+// are 20.5 us.
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
@@ -941,7 +942,8 @@ int launch_cluster(mpc_device *dev, const SampleParams &p, int rows, cudaStream_
 }
 
 // CTAs per row: more than the two that an SM holds, so that the rows under way at a time stay in L2 for the later
-// passes (256 rows of 131071 f32: 2, 4 and 8 CTAs 346, 242 and 232 us), and at least 1024 tokens each.
+// passes (256 rows of 131071 f32: 2, 4 and 8 CTAs 186, 175 and 173 us; 4 rows of 50257 bf16: 19.1, 15.2 and 14.7 us),
+// and at least 1024 tokens each.
 template <int DT>
 int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
   int c = 1;
