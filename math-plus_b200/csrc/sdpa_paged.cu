@@ -549,9 +549,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 //   V: the lane holds values 64 j + 8 r ..+7 of keys 2c, 2c+1, 2c+8, 2c+9; the pairs of neighbouring keys
 //      that the products want are byte permutes of two such registers.
 // Weights: S^T's layout transposed (movmatrix) is P^T's. A weight goes in as the sum of two numbers of the
-// type (its rounding and the rest), which leaves 2^-16 (bf16) or less of it; one number alone would add
-// as much error as the output's own rounding. Over 8-bit rows the weights are f16, and where the output is
-// bf16 their rounding of 2^-12 is an eighth of the output's, so one number does.
+// type (its rounding and the rest), which leaves 2^-16 (bf16) or 2^-22 (f16, the type over 8-bit rows) of it; one
+// number alone would leave 2^-8 or 2^-11, of sum p |v| and not of the output, which is smaller where V cancels.
 // The reference m of the exponentials is only raised when a score passes it by more than 2^kSlack: a warp
 // vote per tile in the common case, the row maximum by shuffles and a rescaling of O else. It is set 2^kHead
 // below the maximum so that small weights stay clear of f16's subnormals.
@@ -639,15 +638,14 @@ __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND
   }
 }
 
-// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value; LO: weights as two
-// numbers. TPI tiles of 16 keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks
+// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value. TPI tiles of 16 keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks
 // per SM as the registers allow; over 8-bit rows of 128 two blocks of 32 keys a warp (94 us at 2 x ~115k keys, the join
 // left out) beat three of 16 (100 us).
 template <int KIND, int DP>
 constexpr int tiles_at_once() { return DP == 64 || (DP == 128 && KIND == kE4M3) ? 2 : 1; }
 constexpr int blocks_per_sm(bool e4m3, int dp, int heads) { return dp == 256 || heads == 16 || (dp == 128 && e4m3) ? 2 : 3; }
 
-template <int KIND, int DP, int NT, int QS, bool LO>
+template <int KIND, int DP, int NT, int QS>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND == kE4M3, DP, 8 * NT)) mma_kernel(const Params p) {
   constexpr bool BF = KIND == kBF16, Q8 = KIND == kE4M3;
   constexpr int KC = DP / 32, VC = DP / 64, GT = 8 * NT, PITCH = DP + 8, TPI = tiles_at_once<KIND, DP>(), KEYS = 16 * TPI;
@@ -908,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND == kE4M3, DP, 8 *
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma<BF>(o[n][j][i], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-              if constexpr (LO) mma<BF>(o[n][j][i], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+              mma<BF>(o[n][j][i], a0, a1, a2, a3, lo[n][0], lo[n][1]);
             }
           }
       }
@@ -991,13 +989,13 @@ static void launch_simt(const Params &p, int ctas, cudaStream_t st) {
   else simt_kernel<NI, 1, VEC><<<ctas, kThreads, 0, st>>>(p);
 }
 
-template <int KIND, int QS, bool LO>
+template <int KIND, int QS>
 static void launch_mma(const Params &p, const Plan &pl, cudaStream_t st) {
   constexpr int NT = QS == 2 ? 1 : 2;
   auto run = [&](auto kern) { kern<<<pl.ctas, kThreads, 0, st>>>(p); };
-  if (pl.dp == 64) pl.gt == 16 ? run(mma_kernel<KIND, 64, NT, QS, LO>) : run(mma_kernel<KIND, 64, 1, QS, LO>);
-  else if (pl.dp == 128) pl.gt == 16 ? run(mma_kernel<KIND, 128, NT, QS, LO>) : run(mma_kernel<KIND, 128, 1, QS, LO>);
-  else run(mma_kernel<KIND, 256, 1, QS, LO>);
+  if (pl.dp == 64) pl.gt == 16 ? run(mma_kernel<KIND, 64, NT, QS>) : run(mma_kernel<KIND, 64, 1, QS>);
+  else if (pl.dp == 128) pl.gt == 16 ? run(mma_kernel<KIND, 128, NT, QS>) : run(mma_kernel<KIND, 128, 1, QS>);
+  else run(mma_kernel<KIND, 256, 1, QS>);
 }
 
 }  // namespace paged
@@ -1070,11 +1068,10 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
   p.dt = desc->dtype, p.dt_pages = cache->dtype, p.scale_log2 = desc->scale * kLog2e;
   const bool vec = aligned && p.d % 8 == 0 && p.dv % 8 == 0;
   const int dm = p.d > p.dv ? p.d : p.dv;
-  if (pl.dp && cache->dtype == MPC_F16) launch_mma<kF16, 1, true>(p, pl, st);
-  else if (pl.dp && cache->dtype == MPC_BF16) launch_mma<kBF16, 1, true>(p, pl, st);
-  else if (pl.dp && desc->dtype == MPC_F32) launch_mma<kE4M3, 2, true>(p, pl, st);
-  else if (pl.dp && desc->dtype == MPC_F16) launch_mma<kE4M3, 1, true>(p, pl, st);
-  else if (pl.dp) launch_mma<kE4M3, 1, false>(p, pl, st);
+  if (pl.dp && cache->dtype == MPC_F16) launch_mma<kF16, 1>(p, pl, st);
+  else if (pl.dp && cache->dtype == MPC_BF16) launch_mma<kBF16, 1>(p, pl, st);
+  else if (pl.dp && desc->dtype == MPC_F32) launch_mma<kE4M3, 2>(p, pl, st);
+  else if (pl.dp) launch_mma<kE4M3, 1>(p, pl, st);
   else if (dm <= 64) vec ? launch_simt<1, true>(p, pl.ctas, st) : launch_simt<1, false>(p, pl.ctas, st);
   else if (dm <= 128) vec ? launch_simt<2, true>(p, pl.ctas, st) : launch_simt<2, false>(p, pl.ctas, st);
   else vec ? launch_simt<4, true>(p, pl.ctas, st) : launch_simt<4, false>(p, pl.ctas, st);

@@ -228,3 +228,15 @@ def test_workspace_of_the_caller_on_another_stream(be):
         with pytest.raises(F.MpcError, match="workspace"):
             call(*args)
     dev.destroy_stream(s)
+
+
+@pytest.mark.parametrize("qd", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [2, 6, 40])
+def test_cancelling_rows_show_the_weights(be, qd, n):
+    """8-bit V rows in pairs (v, -v) under nearly equal weights: the outputs are differences of weights, so that
+    an error of a weight shows against the output's own rounding (a weight of one f16 number would be off by up
+    to 2^-11 of itself; the bound here is about 2^-17 of the rows)."""
+    hc = HostCache(4, 16, 2, 64, 64, "e4m3", seed=n)
+    hc.pages[1][:, :, 1::2] = hc.pages[1][:, :, ::2] ^ 0x80
+    hc.scales[1][:, :, 1::2] = hc.scales[1][:, :, ::2]
+    check(be, 16, qd, "e4m3", 8, 16, 2, 64, 64, [n], seed=n, scale=1.0, host_cache=hc, q_mag=2.0 ** -10)
