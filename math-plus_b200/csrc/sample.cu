@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     bins.top = wt.top, bins.scale = kBinsPerNat / t, bins.lo = bins.hi = 0, bins.shift = 0;
     const bool by_value = fabsf(wt.top) < INFINITY && bins.scale > 0.0f && bins.scale < INFINITY;
     if (!by_value) bins.whole_row(top_key);
-    quick = quick && bound;
+    quick = quick && bound && by_value;  // the bound's gather goes by values
     bool counting = by_k;
     unsigned n_above = 0;     // tokens above the interval
     u64 base = 0;             // their weight

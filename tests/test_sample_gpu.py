@@ -137,3 +137,22 @@ def test_draws_follow_the_weights(be):
     tok = be.read_sync(be.sample(up(be, x.astype(np.float32), "f32"), up(be, u.astype(np.float32), "f32"))).data
     share = np.bincount(tok, minlength=5)
     assert np.all(np.abs(share - np.exp(logits) * n) <= 1.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_small_top_k_without_bins_by_value(be, dtype):
+    """An infinite temperature, one whose inverse leaves f32, an infinite largest logit: the bins are by the logits'
+    bits, and the kept set is the definition's for every top_k."""
+    B, inf = 6, np.inf
+    for vocab in (300, 1000, 20000):
+        x = np.random.default_rng(vocab).standard_normal((B, vocab)) * 3
+        x[:, 7::13] = -inf
+        for k in (1, 2, 50, 192, 193):
+            check(be, x, dtype, uniform(B, k), t=inf, k=k)
+            check(be, x, dtype, uniform(B, k), t=inf, k=k, p=0.7)
+            check(be, x, dtype, uniform(B, k), t=1e-38, k=k)
+        x[:, [3, vocab // 2]] = inf
+        for k in (1, 2, 3, 50, 192):
+            check(be, x, dtype, uniform(B, k), k=k)
+            check(be, x, dtype, uniform(B, k), t=inf, k=k)
+    check(be, np.array([[inf, 1, inf, 2, 0]]), dtype, [0.7], k=4)
