@@ -374,7 +374,8 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
  * the lowest index at which the kept weights' running sum exceeds u times their total. Weights are
  * evaluated in f64 and summed as integers (2^-46 of the largest weight at 2^16 tokens), so the result
  * does not depend on the order of the sum.
- * temperature <= 0 (or NaN): the largest logit, lowest index first. top_k <= 0, top_p >= 1, min_p <= 0: off.
+ * temperature <= 0 (or NaN), or min_p above 1: the largest logit, lowest index first. top_k <= 0, top_p >= 1 or NaN,
+ * min_p <= 0 or NaN: off.
  * NaN logits count as -inf; a row with nothing above -inf gives token -1, prob 0, kept 0. u is clamped
  * to [0, 1) (NaN: 0). */
 typedef struct {

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
   // Lane i reads CTA i: one remote latency.
   top_key = __reduce_max_sync(0xffffffffu, lane < C ? *cl.map_shared_rank(&sm.key_max, lane) : 0u);
   const uint32_t bound = __reduce_min_sync(0xffffffffu, lane < C ? *cl.map_shared_rank(&sm.key_kth, lane) : 0xffffffffu);
-  if (top_key == 0 || !(t > 0.0f)) {
+  if (top_key == 0 || !(t > 0.0f) || min_p > 1.0f) {  // nothing to draw among: with min_p above 1 the first rank is left
     const float top = top_key ? logit_of(top_key) : 0.0f;
     unsigned at = 0xffffffffu;  // its lowest index
     if (top_key) rd.each(v0, v1, [&](float f, int i) {

@@ -905,8 +905,8 @@ class CudaBackend:
         ``top_k``, ``top_p`` and ``min_p`` are numbers or per-row arrays (f32; top_k i32). Ranked by logit (ties:
         lowest index first), the first top_k are kept, of those the ranks before which less than top_p of
         their weight lies, of those the ones at least min_p times the best; the token is the lowest index
-        whose running sum of kept weights exceeds u times their total. temperature <= 0 takes the best token;
-        top_k <= 0, top_p >= 1, min_p <= 0 are off. A row with nothing above -inf gives -1. ``details=True``
+        whose running sum of kept weights exceeds u times their total. temperature <= 0 (or min_p above 1) takes the best
+        token; top_k <= 0, top_p >= 1, min_p <= 0 are off. A row with nothing above -inf gives -1. ``details=True``
         also returns the token's probability in the kept set (f32 [B]) and the set's size (i32 [B])."""
         self._mine("sample", logits)
         if len(logits.shape) != 2 or not logits.shape[1]:

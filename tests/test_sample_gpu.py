@@ -156,3 +156,23 @@ def test_small_top_k_without_bins_by_value(be, dtype):
             check(be, x, dtype, uniform(B, k), k=k)
             check(be, x, dtype, uniform(B, k), t=inf, k=k)
     check(be, np.array([[inf, 1, inf, 2, 0]]), dtype, [0.7], k=4)
+
+
+def test_min_p_above_one_keeps_the_first_rank(be):
+    """No weight reaches a min_p above 1, so the rank that is always kept is left: of equal best logits the lowest
+    index alone."""
+    x = np.random.default_rng(2).standard_normal((4, 5000))
+    x[:, [17, 400, 4999]] = 9.0
+    for m in (1.0 + 2.0 ** -23, 2.0, np.inf):
+        for kw in (dict(), dict(k=2), dict(p=0.9), dict(k=1000, p=0.9)):
+            check(be, x, "f32", [0.0, 0.4, 0.7, 0.999], m=m, **kw)
+    check(be, x, "f32", [0.0, 0.4, 0.7, 0.999], m=1.0)
+    check(be, x, "f32", [0.0, 0.4, 0.7, 0.999], m=[1.0, 2.0, 1.0, 3.0])
+
+
+def test_min_p_where_its_logit_leaves_the_range(be):
+    """t ln(min_p) below f32's range, the logit where min_p lies within it: 3e38 - 4.02e38."""
+    x = np.array([[-2e38, 3e38, -3e38, 0, 2.9e38, -1.1e38, -1e38]])
+    for u in (0.0, 0.02, 0.3, 0.8, 0.95, 0.999):
+        for kw in (dict(), dict(p=0.99), dict(k=6)):
+            check(be, x, "f32", [u], t=1e38, m=0.018, **kw)
