@@ -372,8 +372,8 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
  * first), the kept set is the first top_k ranks, of those the ranks before which less than top_p of the
  * top-k's weight lies, of those the ones with w_i >= min_p; the first rank is always kept. The token is
  * the lowest index at which the kept weights' running sum exceeds u times their total. Weights are
- * evaluated in f64 and summed as integers (2^-46 of the largest weight at 2^16 tokens), so the result
- * does not depend on the order of the sum.
+ * evaluated in f64 and summed as integers (multiples of 2^-46 of the largest weight at 2^16 tokens, 2^-42 at 2^20,
+ * the most that a row may have), so the result does not depend on the order of the sum.
  * temperature <= 0 (or NaN), or min_p above 1: the largest logit, lowest index first. top_k <= 0, top_p >= 1 or NaN,
  * min_p <= 0 or NaN: off.
  * NaN logits count as -inf; a row with nothing above -inf gives token -1, prob 0, kept 0. u is clamped

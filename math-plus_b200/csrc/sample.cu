@@ -19,8 +19,10 @@
 // Rows are read again by each step, from L1 or L2; HBM is read once.
 //
 // Weights w = exp((l - max) / T) in f64 are held as integers of 2^-shift (shift = 62 - log2 of the row's length, at
-// most 51), so that sums are exact whatever their order: the same row always gives the same token, and
-// the borders of top-p and of the drawn interval move by less than 1e-11 of the total.
+// most 51), so that sums are exact whatever their order: the same row always gives the same token. The roundings of V
+// weights move the borders of top-p and of the drawn interval by at most V 2^-(shift + 1) of the largest weight, at
+// worst (a tail of weights just under half a unit): 2^-31 at 2^16 tokens, 2^-23, two steps of u next to 1, at 2^20.
+// Rows of more tokens are refused.
 //
 // A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy. A few rows are bound by latency (cluster
 // barriers and remote reads), many by the instructions per token of the passes, the f64 exponentials (10 double
@@ -968,8 +970,8 @@ extern "C" int mpc_sample(mpc_device *dev, const mpc_sample_desc *d, const void 
   if (d->dtype < MPC_F32 || d->dtype > MPC_BF16) return fail(MPC_ERR_INVALID, "mpc_sample: logits of dtype %d", d->dtype);
   if (d->rows < 0 || d->vocab < 0 || d->row_stride < 0)
     return fail(MPC_ERR_INVALID, "mpc_sample: negative extent or stride");
-  if (d->rows > INT32_MAX || d->vocab > (1 << 30))
-    return fail(MPC_ERR_UNSUPPORTED, "mpc_sample: more than 2^31 - 1 rows or 2^30 tokens");
+  if (d->rows > INT32_MAX || d->vocab > (1 << 20))
+    return fail(MPC_ERR_UNSUPPORTED, "mpc_sample: more than 2^31 - 1 rows or 2^20 tokens");
   if (d->rows == 0) return MPC_OK;
   if (d->vocab == 0) return fail(MPC_ERR_INVALID, "mpc_sample: rows of no tokens");
   if (!logits || !u || !token) return fail(MPC_ERR_INVALID, "mpc_sample: null pointer");

@@ -176,3 +176,19 @@ def test_min_p_where_its_logit_leaves_the_range(be):
     for u in (0.0, 0.02, 0.3, 0.8, 0.95, 0.999):
         for kw in (dict(), dict(p=0.99), dict(k=6)):
             check(be, x, "f32", [u], t=1e38, m=0.018, **kw)
+
+
+def test_vocabularies_beyond_the_sums_are_refused(be):
+    """The weights' fixed point holds 2^20 tokens to 2^-23 of the largest weight; more are refused."""
+    from tensor_cuda import _ffi as F
+    n = 1 << 20
+    x = np.full((1, n + 1), -20.0, np.float16)
+    x[0, 5] = 0
+    u = up(be, np.float32([0.5]), "f32")
+    tok, prob, kept = (be.read_sync(a).data for a in be.sample(up(be, x[:, :n].copy(), "f16"), u, details=True))
+    w = (n - 1) * np.exp(-20.0)
+    # 2^20 weights rounded to 2^-42: 2^-23 of the total at most, and the rounding to f32
+    assert tok[0] == 5 and kept[0] == n and abs(prob[0] - 1 / (1 + w)) <= 2.0 ** -23 + 2.0 ** -24
+    with pytest.raises(F.MpcError, match="2\\^20 tokens") as e:
+        be.sample(up(be, x, "f16"), u)
+    assert e.value.status == F.ERR_UNSUPPORTED
