@@ -52,7 +52,7 @@ struct KvParams {
   void *rows[2];       // the tokens' dense K, V rows (source of an append, destination of a read)
   long long ts[2], hs[2];  // element strides of the rows' token and head axes
   const int32_t *table, *seq, *pos;
-  int *err;
+  unsigned long long *report;
   int d[2];
   int n, n_seq, hk, page_size, n_pages, dt_rows, dt_pages;
   long long max_pages;
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool locate(const KvParams &p, long long t, long long
   int pg = -1;
   if (seq >= 0 && seq < p.n_seq && col < p.max_pages) pg = p.table[(long long)seq * p.max_pages + col];
   if (pg < 0 || pg >= p.n_pages) {
-    if (first) report_bad_page(p.err, kBadAppendRead, (int)t);
+    if (first) report_bad_page(p.report, kBadAppendRead, (int)t);
     return false;
   }
   *page = pg;
@@ -278,7 +278,7 @@ int kv_run(mpc_device *dev, const char *what, const mpc_kv_desc *c, void *k_page
   p.pages[0] = k_pages, p.pages[1] = v_pages, p.scales[0] = k_scale, p.scales[1] = v_scale;
   p.rows[0] = k, p.rows[1] = v;
   p.ts[0] = t->k_stride[0], p.hs[0] = t->k_stride[1], p.ts[1] = t->v_stride[0], p.hs[1] = t->v_stride[1];
-  p.table = table, p.seq = seq, p.pos = pos, p.err = dev->d_err;
+  p.table = table, p.seq = seq, p.pos = pos, p.report = dev->report();
   p.d[0] = (int)c->d, p.d[1] = (int)c->dv;
   p.n = (int)t->n, p.n_seq = (int)t->n_seq, p.hk = (int)c->hk, p.page_size = (int)c->page_size;
   p.n_pages = (int)c->n_pages, p.max_pages = t->max_pages, p.dt_rows = t->dtype, p.dt_pages = c->dtype;

@@ -14,12 +14,12 @@ namespace mpc {
 // Checks of a cache descriptor (kv_cache.cu).
 int kv_check(const char *what, const mpc_kv_desc *c);
 
-// The device's error words: [0] a bounded wait, [1] the kind below, [2] the token or sequence. The
-// next synchronisation reports and clears [1] and [2] (mpc_runtime.cu).
+// A report of a place outside the cache: the kind above the token or sequence, in one word, so that it is left and
+// taken (mpc_runtime.cu) whole. The first one stays until a synchronisation takes it.
 enum : int { kBadAppendRead = 1, kBadAttend = 2, kBadLength = 3 };
 
-__device__ __forceinline__ void report_bad_page(int *err, int kind, int which) {
-  if (atomicCAS(err + 1, 0, kind) == 0) err[2] = which;
+__device__ __forceinline__ void report_bad_page(unsigned long long *report, int kind, int which) {
+  atomicCAS(report, 0ull, (unsigned long long)kind << 32 | (unsigned)which);
 }
 
 // Two e4m3 numbers (low byte first) as f16x2, exactly.

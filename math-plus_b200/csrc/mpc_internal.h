@@ -40,13 +40,15 @@ struct mpc_allocator {
 struct mpc_device {
   int ordinal = -1;
   cudaStream_t stream = nullptr;
-  int *d_err = nullptr;  // kernel error word (device memory)
+  int *d_err = nullptr;  // kernel error word (device memory), and at 8 bytes the report of a place outside a paged cache
+  std::mutex report_mu;  // one thread at a time takes a report
   int *d_counters = nullptr;  // zero between the kernels of `stream` that count in them
   std::atomic<int> sticky{0};
   uint64_t timeout_ns = 2000000000ull;
   std::atomic<uint64_t> launches{0};
   cudaDeviceProp prop{};
   mpc_allocator alloc;
+  unsigned long long *report() const { return reinterpret_cast<unsigned long long *>(d_err) + 1; }
 };
 
 // One rank of an NCCL communicator (comm.cu).

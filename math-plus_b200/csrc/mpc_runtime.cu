@@ -259,9 +259,11 @@ int mpc_device_create(int ordinal, unsigned flags, mpc_device **out) {
     return rc;
   }
   if ((e = cudaStreamCreateWithFlags(&dev->stream, cudaStreamNonBlocking)) != cudaSuccess ||
-      (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess || (e = cudaMemset(dev->d_err, 0, 256)) != cudaSuccess ||
+      (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess ||
+      (e = cudaMemsetAsync(dev->d_err, 0, 256, dev->stream)) != cudaSuccess ||
       (e = cudaMalloc(&dev->d_counters, kCounterBytes)) != cudaSuccess ||
-      (e = cudaMemsetAsync(dev->d_counters, 0, kCounterBytes, dev->stream)) != cudaSuccess) {
+      (e = cudaMemsetAsync(dev->d_counters, 0, kCounterBytes, dev->stream)) != cudaSuccess ||
+      (e = cudaStreamSynchronize(dev->stream)) != cudaSuccess) {  // zero before any stream's kernel
     rc = cuda_fail(nullptr, e, "mpc_device_create");
     if (dev->d_err) cudaFree(dev->d_err);
     if (dev->d_counters) cudaFree(dev->d_counters);
@@ -436,43 +438,55 @@ int mpc_device_stream(mpc_device *dev, mpc_stream *s) {
   return MPC_OK;
 }
 
-static int read_error_word(mpc_device *dev) {
-  int word[3] = {0, 0, 0};
-  cudaError_t e = cudaMemcpy(word, dev->d_err, sizeof(word), cudaMemcpyDeviceToHost);
+// taken = report, report = 0: in one step on the device, so that what a kernel reports meanwhile is either taken or stays.
+static __global__ void take_report_kernel(unsigned long long *report, unsigned long long *taken) {
+  *taken = atomicExch(report, 0ull);
+}
+
+// The error words, after `st` has been synchronised; a report is taken on `st`.
+static int read_error_word(mpc_device *dev, cudaStream_t st) {
+  unsigned long long words[2] = {0, 0};
+  cudaError_t e = cudaMemcpy(words, dev->d_err, sizeof(words), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(dev, e, "reading the kernel error word");
-  if (word[0]) {
+  if (const int site = (int)words[0]) {
     dev->sticky = MPC_ERR_TIMEOUT;
-    return fail(MPC_ERR_TIMEOUT, "a kernel's bounded wait ran out (site 0x%x); its results are invalid", word[0]);
+    return fail(MPC_ERR_TIMEOUT, "a kernel's bounded wait ran out (site 0x%x); its results are invalid", site);
   }
-  if (word[1]) {  // the kernel left the access out and went on, so the handle stays usable: report once
-    MPC_CUDA(dev, cudaMemset(dev->d_err + 1, 0, 2 * sizeof(int)));
-    switch (word[1]) {
-      case kBadAppendRead:
-        return fail(MPC_ERR_INVALID, "paged cache: token %d names a sequence, position or page outside the cache",
-                    word[2]);
-      case kBadAttend:
-        return fail(MPC_ERR_INVALID, "paged cache: the block table of sequence %d names a page outside the cache",
-                    word[2]);
-      default:
-        return fail(MPC_ERR_INVALID, "paged cache: the length of sequence %d is negative or beyond its block table",
-                    word[2]);
-    }
+  if (!words[1]) return MPC_OK;
+  // The kernel left the access out and went on, so the handle stays usable: report once.
+  unsigned long long taken = 0;
+  {
+    std::lock_guard<std::mutex> lk(dev->report_mu);
+    take_report_kernel<<<1, 1, 0, st>>>(dev->report(), dev->report() + 1);
+    MPC_CUDA(dev, cudaGetLastError());
+    MPC_CUDA(dev, cudaMemcpyAsync(&taken, dev->report() + 1, sizeof(taken), cudaMemcpyDeviceToHost, st));
+    MPC_CUDA(dev, cudaStreamSynchronize(st));
   }
-  return MPC_OK;
+  const int which = (int)(unsigned)taken;
+  switch ((int)(taken >> 32)) {
+    case 0:  // another thread's synchronisation has taken it
+      return MPC_OK;
+    case kBadAppendRead:
+      return fail(MPC_ERR_INVALID, "paged cache: token %d names a sequence, position or page outside the cache", which);
+    case kBadAttend:
+      return fail(MPC_ERR_INVALID, "paged cache: the block table of sequence %d names a page outside the cache", which);
+    default:
+      return fail(MPC_ERR_INVALID, "paged cache: the length of sequence %d is negative or beyond its block table", which);
+  }
 }
 
 int mpc_stream_sync(mpc_device *dev, mpc_stream s) {
   int rc = enter(dev);
   if (rc) return rc;
   MPC_CUDA(dev, cudaStreamSynchronize(stream_of(dev, s)));
-  return read_error_word(dev);
+  return read_error_word(dev, stream_of(dev, s));
 }
 
 int mpc_sync(mpc_device *dev) {
   int rc = enter(dev);
   if (rc) return rc;
   MPC_CUDA(dev, cudaDeviceSynchronize());
-  return read_error_word(dev);
+  return read_error_word(dev, dev->stream);
 }
 
 int mpc_event_create(mpc_device *dev, mpc_event *e) {
@@ -525,7 +539,8 @@ int mpc_device_clear_error(mpc_device *dev) {
   int rc = enter(dev);
   if (rc) return rc;
   MPC_CUDA(dev, cudaDeviceSynchronize());
-  MPC_CUDA(dev, cudaMemset(dev->d_err, 0, 256));
+  MPC_CUDA(dev, cudaMemsetAsync(dev->d_err, 0, 256, dev->stream));
+  MPC_CUDA(dev, cudaStreamSynchronize(dev->stream));
   dev->sticky = MPC_OK;
   return MPC_OK;
 }

@@ -47,7 +47,7 @@ struct Params {
   void *out;
   float *lse, *ws;
   int *counters;  // per warp: the warps that have left their part of the item that it starts
-  int *err;
+  unsigned long long *report;
   long long qs[2], os[2], max_pages, cap;  // cap: max_pages * page_size
   int B, H, hk, group, gt, qt, tile;  // query heads per K/V head, per query tile; tiles per K/V head; keys of a tile
   int d, dv, page_size, n_pages, dt, dt_pages;
@@ -163,7 +163,7 @@ __device__ __forceinline__ float guard_exp2(float x, float ref) { return x == -I
 __device__ __forceinline__ void empty_rows(const Params &p) {
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     const int len = p.lengths[b];
-    if (threadIdx.x == 0 && (len < 0 || len > p.cap)) report_bad_page(p.err, kBadLength, b);
+    if (threadIdx.x == 0 && (len < 0 || len > p.cap)) report_bad_page(p.report, kBadLength, b);
     if (len > 0 && p.cap > 0) continue;
     for (int i = threadIdx.x; i < p.H * p.dv; i += kThreads) {
       const int h = i / p.dv;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
       const unsigned col = p.page_of(key);
       const int pg = p.table[(long long)b * p.max_pages + col];
       if (pg >= 0 && pg < p.n_pages) return ((long long)pg * p.hk + kvh) * p.page_size + (key - col * (unsigned)p.page_size);
-      if ((lane & 7) == 0) report_bad_page(p.err, kBadAttend, b);
+      if ((lane & 7) == 0) report_bad_page(p.report, kBadAttend, b);
       return -1;
     };
     // Where the registers allow, a key's V and the next step's row are under way with its K.
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KIND == kE4M3, DP, 8 *
       const unsigned col = p.page_of(key);
       const int pg = __ldg(table + col);
       if (pg < 0 || pg >= p.n_pages) {
-        report_bad_page(p.err, kBadAttend, b);
+        report_bad_page(p.report, kBadAttend, b);
         return kNoRow;
       }
       return ((unsigned)pg * (unsigned)p.hk + kvh) * (unsigned)p.page_size + (key - col * (unsigned)p.page_size);
@@ -1052,7 +1052,7 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
   }
   Params p{};
   p.q = Q, p.kp = k_pages, p.vp = v_pages, p.ks = k_scale, p.vs = v_scale, p.table = table, p.lengths = lengths;
-  p.out = O, p.lse = LSE, p.err = dev->d_err, p.tile = pl.tile, p.counters = counters;
+  p.out = O, p.lse = LSE, p.report = dev->report(), p.tile = pl.tile, p.counters = counters;
   p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + pl.counters_bytes);
   for (int i = 0; i < 2; ++i) p.qs[i] = desc->q_stride[i], p.os[i] = desc->o_stride[i];
   p.max_pages = desc->max_pages, p.cap = desc->max_pages * cache->page_size;

@@ -196,3 +196,42 @@ def test_dtype_of_the_dense_rows_is_kept(be):
     k, _ = be.kv_read(c, up_quietly(be, [[0]]), up_quietly(be, [2]))
     assert k.dtype == "bf16"
     assert np.array_equal(from_storage(be.read_sync(k).data.reshape(1, 1, 8), "bf16")[0], h.values(0)[0, :, 2])
+
+
+class Appends:
+    """kv_append of one token on a stream of one's choice, to a good or a bad place; pool memory that is only written."""
+
+    def __init__(self, be):
+        from tensor_cuda import _ffi as F
+        self.be, self.F = be, F
+        self.cache = HostCache(2, 4, 1, 16, 16, "f16").upload(be)
+        self.x = up(be, np.ones((1, 1, 16), np.float16), "f16")
+        self.table, self.zero = up_quietly(be, [[0, 7]]), up_quietly(be, [0])
+        self.bad = up_quietly(be, [4])  # in page 7 of 2
+        self.tokens = F.KvTokens(1, 1, 2, F.I64x2(16, 16), F.I64x2(16, 16), F.F16, 0)
+
+    def call(self, stream, pos):
+        import ctypes as C
+        self.F.call("mpc_kv_append", self.be.device.handle, *self.cache.args, C.byref(self.tokens), C.c_void_p(self.x.ptr),
+                    C.c_void_p(self.x.ptr), C.c_void_p(self.table.ptr), C.c_void_p(self.zero.ptr), C.c_void_p(pos.ptr),
+                    C.c_void_p(stream))
+
+    def reports(self, sync):
+        try:
+            sync()
+        except self.F.MpcError as e:
+            assert e.status == self.F.ERR_INVALID and "token 0" in str(e)
+            return True
+        return False
+
+
+def test_every_bad_call_is_reported(be):
+    """A call right behind a synchronisation that reported: its own report is not wiped by the clearing of the last."""
+    a, dev = Appends(be), be.device
+    s = dev.new_stream()
+    for _ in range(300):
+        for st in (None, s):
+            a.call(st, a.bad)
+            assert a.reports(lambda: dev.stream_sync(st))
+    assert not a.reports(dev.sync)
+    dev.destroy_stream(s)
