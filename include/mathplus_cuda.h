@@ -314,7 +314,10 @@ int mpc_mean_pool(mpc_device *dev, const void *x, int32_t dtype, const void *mas
  * scale byte per (page, head, row) in k_scale / v_scale [n_pages, hk, page_size]: the row's value is
  * code * 2^(byte - 127), the byte the least one whose scaled row stays within 448 (infinities saturate,
  * NaN stays). Head dims up to 256. A token whose sequence, position or page lies outside the cache is
- * left out by the kernel, and the next synchronisation returns MPC_ERR_INVALID naming it (once). */
+ * left out by the kernel, and the next synchronisation of its stream (mpc_stream_sync) or of the device (mpc_sync)
+ * returns MPC_ERR_INVALID naming it (the first of them, once). A call captured into a graph, which may be launched into
+ * any stream, reports to whichever synchronisation comes next; so do streams beyond 126 with such calls (destroyed ones
+ * count until mpc_sync). A stream destroyed before its report was taken leaves it to mpc_sync. */
 typedef struct {
   int64_t n_pages, page_size, hk, d, dv;
   int32_t dtype; /* MPC_F32, MPC_F16, MPC_BF16 or MPC_E4M3 */
@@ -349,7 +352,7 @@ int mpc_kv_read(mpc_device *dev, const mpc_kv_desc *cache, const void *k_pages, 
  * split along the cache by the lengths found on the device; the partial results live in the workspace
  * until the block that completes an item joins them. An infinity or a NaN in a row within the length makes the
  * values that depend on it NaN or infinite, which of the two is not defined. A length that is negative or beyond max_pages * page_size, or a
- * page outside the cache, is cut off or left out, and the next synchronisation returns MPC_ERR_INVALID. */
+ * page outside the cache, is cut off or left out, and reported like a token's place outside the cache. */
 typedef struct {
   int64_t b, h, max_pages;
   int64_t q_stride[2], o_stride[2];

@@ -278,7 +278,8 @@ int kv_run(mpc_device *dev, const char *what, const mpc_kv_desc *c, void *k_page
   p.pages[0] = k_pages, p.pages[1] = v_pages, p.scales[0] = k_scale, p.scales[1] = v_scale;
   p.rows[0] = k, p.rows[1] = v;
   p.ts[0] = t->k_stride[0], p.hs[0] = t->k_stride[1], p.ts[1] = t->v_stride[0], p.hs[1] = t->v_stride[1];
-  p.table = table, p.seq = seq, p.pos = pos, p.report = dev->report();
+  p.table = table, p.seq = seq, p.pos = pos;
+  if ((rc = report_word(dev, st, &p.report))) return rc;
   p.d[0] = (int)c->d, p.d[1] = (int)c->dv;
   p.n = (int)t->n, p.n_seq = (int)t->n_seq, p.hk = (int)c->hk, p.page_size = (int)c->page_size;
   p.n_pages = (int)c->n_pages, p.max_pages = t->max_pages, p.dt_rows = t->dtype, p.dt_pages = c->dtype;

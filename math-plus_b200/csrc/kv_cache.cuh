@@ -15,7 +15,7 @@ namespace mpc {
 int kv_check(const char *what, const mpc_kv_desc *c);
 
 // A report of a place outside the cache: the kind above the token or sequence, in one word, so that it is left and
-// taken (mpc_runtime.cu) whole. The first one stays until a synchronisation takes it.
+// taken (mpc_runtime.cu) whole. A stream's first one stays until a synchronisation takes it.
 enum : int { kBadAppendRead = 1, kBadAttend = 2, kBadLength = 3 };
 
 __device__ __forceinline__ void report_bad_page(unsigned long long *report, int kind, int which) {

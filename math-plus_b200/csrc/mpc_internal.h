@@ -37,18 +37,29 @@ struct mpc_allocator {
   size_t in_use = 0, cached = 0, limit = 0;
 };
 
+// The words in which kernels report places outside a paged cache, one per stream, so that a synchronisation reports
+// the calls it has waited for: word 0 is for captured calls (a graph may be launched into any stream) and for streams
+// beyond the words, word 1 for the device's own stream. A destroyed stream's word is not given to another stream before
+// the whole device has been waited for.
+struct mpc_reports {
+  static constexpr int kWords = 128;
+  std::mutex mu;
+  std::unordered_map<cudaStream_t, int> of;  // the other streams'
+  std::vector<int> free, orphans;
+  int used = 2;  // words handed out so far
+};
+
 struct mpc_device {
   int ordinal = -1;
   cudaStream_t stream = nullptr;
-  int *d_err = nullptr;  // kernel error word (device memory), and at 8 bytes the report of a place outside a paged cache
-  std::mutex report_mu;  // one thread at a time takes a report
+  int *d_err = nullptr;  // kernel error word (device memory), then the reports below
+  mpc_reports reports;
   int *d_counters = nullptr;  // zero between the kernels of `stream` that count in them
   std::atomic<int> sticky{0};
   uint64_t timeout_ns = 2000000000ull;
   std::atomic<uint64_t> launches{0};
   cudaDeviceProp prop{};
   mpc_allocator alloc;
-  unsigned long long *report() const { return reinterpret_cast<unsigned long long *>(d_err) + 1; }
 };
 
 // One rank of an NCCL communicator (comm.cu).
@@ -62,6 +73,7 @@ struct mpc_comm {
 namespace mpc {
 
 constexpr size_t kCounterBytes = 16384;  // of mpc_device::d_counters
+constexpr size_t kErrBytes = 8 * (2 + mpc_reports::kWords);  // of mpc_device::d_err; the last word: a report being taken
 
 // Thread-local last-error text and the helpers that fill it.
 void set_error(const char *fmt, ...);
@@ -78,6 +90,9 @@ int cuda_fail(mpc_device *dev, cudaError_t e, const char *what);
 int enter(mpc_device *dev);
 cudaStream_t stream_of(mpc_device *dev, mpc_stream s);
 int check_launch(mpc_device *dev, const char *what);
+
+// Where kernels queued on `st` report places outside a paged cache.
+int report_word(mpc_device *dev, cudaStream_t st, unsigned long long **word);
 
 // Returns a block to the device cache once the work queued on `st` so far has finished.
 int free_on(mpc_device *dev, void *ptr, cudaStream_t st);

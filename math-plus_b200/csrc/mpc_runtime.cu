@@ -73,6 +73,28 @@ int check_launch(mpc_device *dev, const char *what) {
   return MPC_OK;
 }
 
+int report_word(mpc_device *dev, cudaStream_t st, unsigned long long **word) {
+  mpc_reports &r = dev->reports;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  MPC_CUDA(dev, cudaStreamIsCapturing(st, &cs));
+  int at = 0;
+  if (cs == cudaStreamCaptureStatusNone && st == dev->stream) {
+    at = 1;
+  } else if (cs == cudaStreamCaptureStatusNone) {
+    std::lock_guard<std::mutex> lk(r.mu);
+    auto it = r.of.find(st);
+    if (it != r.of.end()) {
+      at = it->second;
+    } else {
+      if (!r.free.empty()) at = r.free.back(), r.free.pop_back();
+      else if (r.used < mpc_reports::kWords) at = r.used++;
+      if (at) r.of.emplace(st, at);
+    }
+  }
+  *word = reinterpret_cast<unsigned long long *>(dev->d_err) + 1 + at;
+  return MPC_OK;
+}
+
 int free_on(mpc_device *dev, void *ptr, cudaStream_t st) {
   if (!ptr) return MPC_OK;
   mpc_allocator &a = dev->alloc;
@@ -259,8 +281,8 @@ int mpc_device_create(int ordinal, unsigned flags, mpc_device **out) {
     return rc;
   }
   if ((e = cudaStreamCreateWithFlags(&dev->stream, cudaStreamNonBlocking)) != cudaSuccess ||
-      (e = cudaMalloc(&dev->d_err, 256)) != cudaSuccess ||
-      (e = cudaMemsetAsync(dev->d_err, 0, 256, dev->stream)) != cudaSuccess ||
+      (e = cudaMalloc(&dev->d_err, kErrBytes)) != cudaSuccess ||
+      (e = cudaMemsetAsync(dev->d_err, 0, kErrBytes, dev->stream)) != cudaSuccess ||
       (e = cudaMalloc(&dev->d_counters, kCounterBytes)) != cudaSuccess ||
       (e = cudaMemsetAsync(dev->d_counters, 0, kCounterBytes, dev->stream)) != cudaSuccess ||
       (e = cudaStreamSynchronize(dev->stream)) != cudaSuccess) {  // zero before any stream's kernel
@@ -429,7 +451,17 @@ int mpc_stream_create(mpc_device *dev, mpc_stream *s) {
 int mpc_stream_destroy(mpc_device *dev, mpc_stream s) {
   int rc = enter(dev);
   if (rc) return rc;
-  if (s) MPC_CUDA(dev, cudaStreamDestroy(static_cast<cudaStream_t>(s)));
+  if (!s) return MPC_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(s);
+  {
+    std::lock_guard<std::mutex> lk(dev->reports.mu);
+    auto it = dev->reports.of.find(st);
+    if (it != dev->reports.of.end()) {
+      dev->reports.orphans.push_back(it->second);
+      dev->reports.of.erase(it);
+    }
+  }
+  MPC_CUDA(dev, cudaStreamDestroy(st));
   return MPC_OK;
 }
 int mpc_device_stream(mpc_device *dev, mpc_stream *s) {
@@ -443,23 +475,40 @@ static __global__ void take_report_kernel(unsigned long long *report, unsigned l
   *taken = atomicExch(report, 0ull);
 }
 
-// The error words, after `st` has been synchronised; a report is taken on `st`.
-static int read_error_word(mpc_device *dev, cudaStream_t st) {
-  unsigned long long words[2] = {0, 0};
-  cudaError_t e = cudaMemcpy(words, dev->d_err, sizeof(words), cudaMemcpyDeviceToHost);
+// The error words, after `st` has been waited for: its own report and the shared word's, or, with `whole`, after the
+// whole device has been, any. One is taken (on `st`), the others stay for later synchronisations.
+static int read_error_word(mpc_device *dev, cudaStream_t st, bool whole) {
+  mpc_reports &r = dev->reports;
+  unsigned long long words[1 + mpc_reports::kWords] = {};
+  int own = 0, used;
+  {
+    std::lock_guard<std::mutex> lk(r.mu);
+    used = r.used;
+    if (st == dev->stream) {
+      own = 1;
+    } else {
+      auto it = r.of.find(st);
+      if (it != r.of.end()) own = it->second;
+    }
+  }
+  cudaError_t e = cudaMemcpy(words, dev->d_err, (1 + used) * sizeof(words[0]), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(dev, e, "reading the kernel error word");
   if (const int site = (int)words[0]) {
     dev->sticky = MPC_ERR_TIMEOUT;
     return fail(MPC_ERR_TIMEOUT, "a kernel's bounded wait ran out (site 0x%x); its results are invalid", site);
   }
-  if (!words[1]) return MPC_OK;
+  int at = words[1 + own] ? own : words[1] ? 0 : -1;
+  for (int i = 0; whole && at < 0 && i < used; ++i)
+    if (words[1 + i]) at = i;
+  if (at < 0) return MPC_OK;
   // The kernel left the access out and went on, so the handle stays usable: report once.
   unsigned long long taken = 0;
   {
-    std::lock_guard<std::mutex> lk(dev->report_mu);
-    take_report_kernel<<<1, 1, 0, st>>>(dev->report(), dev->report() + 1);
+    std::lock_guard<std::mutex> lk(r.mu);  // one thread at a time takes a report
+    unsigned long long *const all = reinterpret_cast<unsigned long long *>(dev->d_err), *const last = all + 1 + mpc_reports::kWords;
+    take_report_kernel<<<1, 1, 0, st>>>(all + 1 + at, last);
     MPC_CUDA(dev, cudaGetLastError());
-    MPC_CUDA(dev, cudaMemcpyAsync(&taken, dev->report() + 1, sizeof(taken), cudaMemcpyDeviceToHost, st));
+    MPC_CUDA(dev, cudaMemcpyAsync(&taken, last, sizeof(taken), cudaMemcpyDeviceToHost, st));
     MPC_CUDA(dev, cudaStreamSynchronize(st));
   }
   const int which = (int)(unsigned)taken;
@@ -479,14 +528,26 @@ int mpc_stream_sync(mpc_device *dev, mpc_stream s) {
   int rc = enter(dev);
   if (rc) return rc;
   MPC_CUDA(dev, cudaStreamSynchronize(stream_of(dev, s)));
-  return read_error_word(dev, stream_of(dev, s));
+  return read_error_word(dev, stream_of(dev, s), false);
 }
 
 int mpc_sync(mpc_device *dev) {
   int rc = enter(dev);
   if (rc) return rc;
-  MPC_CUDA(dev, cudaDeviceSynchronize());
-  return read_error_word(dev, dev->stream);
+  mpc_reports &r = dev->reports;
+  std::vector<int> gone;
+  {
+    std::lock_guard<std::mutex> lk(r.mu);
+    gone.swap(r.orphans);
+  }
+  const cudaError_t e = cudaDeviceSynchronize();
+  rc = e == cudaSuccess ? read_error_word(dev, dev->stream, true) : cuda_fail(dev, e, "cudaDeviceSynchronize()");
+  // Destroyed streams' words: nothing can report there any more, so they are free once nothing is left in them, which
+  // a synchronisation without a report shows.
+  std::lock_guard<std::mutex> lk(r.mu);
+  std::vector<int> &to = rc == MPC_OK ? r.free : r.orphans;
+  to.insert(to.end(), gone.begin(), gone.end());
+  return rc;
 }
 
 int mpc_event_create(mpc_device *dev, mpc_event *e) {
@@ -539,7 +600,7 @@ int mpc_device_clear_error(mpc_device *dev) {
   int rc = enter(dev);
   if (rc) return rc;
   MPC_CUDA(dev, cudaDeviceSynchronize());
-  MPC_CUDA(dev, cudaMemsetAsync(dev->d_err, 0, 256, dev->stream));
+  MPC_CUDA(dev, cudaMemsetAsync(dev->d_err, 0, kErrBytes, dev->stream));
   MPC_CUDA(dev, cudaStreamSynchronize(dev->stream));
   dev->sticky = MPC_OK;
   return MPC_OK;

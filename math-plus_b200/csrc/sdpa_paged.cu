@@ -1052,8 +1052,9 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
   }
   Params p{};
   p.q = Q, p.kp = k_pages, p.vp = v_pages, p.ks = k_scale, p.vs = v_scale, p.table = table, p.lengths = lengths;
-  p.out = O, p.lse = LSE, p.report = dev->report(), p.tile = pl.tile, p.counters = counters;
+  p.out = O, p.lse = LSE, p.tile = pl.tile, p.counters = counters;
   p.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + pl.counters_bytes);
+  if ((rc = report_word(dev, st, &p.report))) return rc;
   for (int i = 0; i < 2; ++i) p.qs[i] = desc->q_stride[i], p.os[i] = desc->o_stride[i];
   p.max_pages = desc->max_pages, p.cap = desc->max_pages * cache->page_size;
   p.B = (int)desc->b, p.H = (int)desc->h, p.hk = (int)cache->hk, p.group = p.H / p.hk, p.gt = pl.gt, p.qt = pl.qt;

@@ -235,3 +235,68 @@ def test_every_bad_call_is_reported(be):
             assert a.reports(lambda: dev.stream_sync(st))
     assert not a.reports(dev.sync)
     dev.destroy_stream(s)
+
+
+def test_a_bad_place_is_reported_to_its_own_stream(be):
+    """The synchronisation of a stream reports that stream's calls; the device's reports any, each once."""
+    a, dev = Appends(be), be.device
+    s, t = dev.new_stream(), dev.new_stream()
+    of = lambda st: a.reports(lambda: dev.stream_sync(st))  # noqa: E731
+    try:
+        a.call(s, a.bad)
+        a.call(t, a.zero)
+        dev.stream_sync(t)
+        assert not of(t) and not of(None) and of(s) and not of(s)
+        a.call(None, a.bad)
+        assert not of(s) and of(None) and not of(None)
+        a.call(s, a.bad)
+        a.call(t, a.bad)
+        assert a.reports(dev.sync) and a.reports(dev.sync) and not a.reports(dev.sync) and not of(s) and not of(t)
+        a.call(s, a.bad)
+        a.call(t, a.bad)
+        assert of(t) and a.reports(dev.sync) and not of(s)
+    finally:
+        dev.destroy_stream(s)
+        dev.destroy_stream(t)
+
+
+def test_bad_places_of_a_destroyed_stream_and_of_many_streams(be):
+    """A stream destroyed before it was synchronised leaves its report to the device's synchronisation, not to a
+    stream created later; more streams than the table of reports holds still report every one."""
+    a, dev = Appends(be), be.device
+    s = dev.new_stream()
+    a.call(s, a.bad)
+    dev.destroy_stream(s)
+    later = [dev.new_stream() for _ in range(4)]
+    for st in later:
+        a.call(st, a.zero)
+        assert not a.reports(lambda: dev.stream_sync(st))
+        dev.destroy_stream(st)
+    assert a.reports(dev.sync) and not a.reports(dev.sync)
+    for _ in range(1200):  # places are handed on
+        st = dev.new_stream()
+        a.call(st, a.zero)
+        dev.destroy_stream(st)
+    many = [dev.new_stream() for _ in range(300)]
+    for st in many:
+        a.call(st, a.bad)
+        assert a.reports(lambda: dev.stream_sync(st)) and not a.reports(lambda: dev.stream_sync(st))
+    for st in many:
+        dev.destroy_stream(st)
+    assert not a.reports(dev.sync)
+
+
+def test_a_captured_call_reports_to_the_next_synchronisation(be):
+    """A graph may be launched into any stream: its reports go to whichever synchronisation comes next."""
+    import torch
+    a, dev = Appends(be), be.device
+    st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=st):
+        a.call(st.cuda_stream, a.bad)
+    other = dev.new_stream()
+    for sync in (dev.sync, dev.stream_sync, lambda: dev.stream_sync(other)):
+        g.replay()
+        torch.cuda.synchronize()
+        assert a.reports(sync) and not a.reports(dev.sync)
+    dev.destroy_stream(other)
