@@ -899,6 +899,24 @@ class CudaBackend:
                None if z is None else z.ptr, None, 0, None)
         return (o, z) if lse else o
 
+    def _sample_settings(self, desc, B: int, **settings) -> list:
+        """Checks settings of B rows: numbers go into ``desc``; the device addresses of per-row arrays, else None."""
+        per_row = []
+        for name, x in settings.items():
+            dt = "i32" if name == "top_k" else "f32"
+            if isinstance(x, CudaTensor):
+                self._mine("sample", x)
+                if x.shape != (B,) or x.dtype != dt:
+                    raise TypeError(f"tensor-cuda: sample: {name} is {dt} [{B}], got {x.dtype} "
+                                    f"[{','.join(map(str, x.shape))}]")
+                per_row.append(x.ptr)
+            else:
+                if name == "top_k":
+                    x = min(int(x), 0x7FFFFFFF) if x > 0 else 0
+                setattr(desc, name, x)
+                per_row.append(None)
+        return per_row
+
     def sample(self, logits: CudaTensor, u: CudaTensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                details: bool = False, out=None):
         """One token per row of logits [B, V] from the uniform numbers u f32 [B]: i32 [B]. ``temperature``,
@@ -914,23 +932,10 @@ class CudaBackend:
         if logits.dtype not in FLOAT:
             raise TypeError(f"tensor-cuda: sample: float logits only, got {logits.dtype}")
         B, V = logits.shape
+        if not isinstance(u, CudaTensor):
+            raise TypeError("tensor-cuda: sample: u is an f32 array, one uniform number per row")
         desc = F.SampleDesc(B, V, V, F.DTYPE_CODES[logits.dtype])
-        per_row = []
-        for name, x, dt in (("u", u, "f32"), ("temperature", temperature, "f32"), ("top_k", top_k, "i32"),
-                            ("top_p", top_p, "f32"), ("min_p", min_p, "f32")):
-            if isinstance(x, CudaTensor):
-                self._mine("sample", x)
-                if x.shape != (B,) or x.dtype != dt:
-                    raise TypeError(f"tensor-cuda: sample: {name} is {dt} [{B}], got {x.dtype} "
-                                    f"[{','.join(map(str, x.shape))}]")
-                per_row.append(x.ptr)
-            elif name == "u":
-                raise TypeError("tensor-cuda: sample: u is an f32 array, one uniform number per row")
-            else:
-                if name == "top_k":
-                    x = min(int(x), 0x7FFFFFFF) if x > 0 else 0
-                setattr(desc, name, x)
-                per_row.append(None)
+        per_row = self._sample_settings(desc, B, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         if out is None:
             outs = [self._alloc((B,), "i32")] + ([self._alloc((B,), "f32"), self._alloc((B,), "i32")] if details else [])
         else:

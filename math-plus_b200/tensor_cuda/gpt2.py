@@ -21,6 +21,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from . import _ffi as F
 from .backend import CudaBackend, CudaTensor, host
 from .kv_cache import BlockTable, PagedKVCache
 
@@ -283,8 +284,8 @@ class GPT2Session:
         """Continues every prompt (a list of token lists, one per sequence) by ``max_new`` tokens drawn with
         ``CudaBackend.sample`` from the uniform numbers u [n_seq, max_new] (none needed with temperature 0: the
         best token). Returns the new tokens. The session goes on from there; the last token drawn has not been
-        fed yet, so the next ids begin with it. Pages for all of it are taken first: when the pool or the context
-        is too small nothing has changed."""
+        fed yet, so the next ids begin with it. Settings are checked and pages for all of it are taken first: when a
+        setting is refused, or the pool or the context is too small, nothing has changed."""
         be, n_ctx = self.model.backend, self.model.cfg.n_ctx
         if len(prompts) != self.n_seq or not all(len(p) for p in prompts):
             raise ValueError(f"GPT2Session: {len(prompts)} prompts for {self.n_seq} sequences, none of them empty")
@@ -295,6 +296,7 @@ class GPT2Session:
         u = np.asarray(u, np.float32)
         if u.shape != (self.n_seq, max_new):
             raise ValueError(f"GPT2Session: u [{','.join(map(str, u.shape))}] for {self.n_seq} sequences of {max_new} tokens")
+        be._sample_settings(F.SampleDesc(), self.n_seq, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         if max_new:
             after = [s + len(p) + max_new - 1 for s, p in zip(self.lengths, prompts)]
             if max(after) > n_ctx:

@@ -146,3 +146,27 @@ def test_generate_takes_all_or_nothing(setup):
     assert s.lengths == [0]
     assert len(s.generate([[1] * 200], 57, temperature=0.0)[0]) == 57 and s.lengths == [256]
     s.dispose()
+
+
+def test_generate_refuses_settings_before_it_steps(setup):
+    """Settings that sample would refuse are refused while nothing has changed."""
+    from tensor_cuda.backend import host
+    be, cfg, w, model = setup
+    s = model.session(2)
+    free = s.table.free_pages
+    u = np.full((2, 3), 0.5)
+    wrong = be.from_host_sync(host("f32", (3,), np.ones(3, np.float32)))
+    whole = be.from_host_sync(host("i32", (2,), np.ones(2, np.int32)))
+    for kw in (dict(temperature=wrong), dict(top_k=wrong), dict(top_p=whole), dict(min_p=wrong), dict(temperature=None),
+               dict(top_p="0.9"), dict(top_k=[1, 2])):
+        with pytest.raises((TypeError, ValueError)):
+            s.generate([[1, 2, 3], [4]], 3, u, **kw)
+        assert s.lengths == [0, 0] and s.table.free_pages == free
+    gone = be.from_host_sync(host("f32", (2,), np.ones(2, np.float32)))
+    be.dispose(gone)
+    with pytest.raises(RuntimeError, match="dispose"):
+        s.generate([[1, 2, 3], [4]], 3, u, top_p=gone)
+    assert s.lengths == [0, 0] and s.table.free_pages == free
+    a = s.generate([[1, 2, 3], [4]], 3, u, temperature=1.0, top_k=whole)
+    assert [len(x) for x in a] == [3, 3] and s.lengths == [5, 3]
+    s.dispose()
