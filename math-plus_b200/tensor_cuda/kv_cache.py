@@ -116,8 +116,8 @@ class BlockTable:
 
     @property
     def device(self):
-        """The table on the device (uploaded after a change)."""
-        if self._device is None:
+        """The table on the device (uploaded after a change, or where a scope has released it)."""
+        if self._device is None or self._device.disposed:
             from .backend import host
             self._device = self.backend.from_host_sync(host("i32", self.host.shape, self.host))
         return self._device

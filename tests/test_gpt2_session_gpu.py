@@ -170,3 +170,16 @@ def test_generate_refuses_settings_before_it_steps(setup):
     a = s.generate([[1, 2, 3], [4]], 3, u, temperature=1.0, top_k=whole)
     assert [len(x) for x in a] == [3, 3] and s.lengths == [5, 3]
     s.dispose()
+
+
+def test_a_session_inside_a_scope(setup):
+    """Steps within be.scope keep the session usable behind it; the logits returned are the caller's."""
+    be, cfg, w, model = setup
+    ids = O.randint_i32(2 * 30, 9, cfg.vocab).reshape(2, 30)
+    s = model.session(2)
+    first = be.scope(lambda: s.step(ids[:, :20]))
+    check(cfg, w, ids, [20, 20], read(be, first))
+    check(cfg, w, ids, [21, 21], read(be, s.step(ids[:, 20:21])))
+    check(cfg, w, ids, [24, 24], read(be, be.scope(lambda: s.step(ids[:, 21:24]))))
+    check(cfg, w, ids, [25, 25], read(be, s.step(ids[:, 24:25])))
+    s.dispose()

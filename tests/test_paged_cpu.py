@@ -187,3 +187,23 @@ def test_eight_bit_arithmetic_of_the_tests():
     codes, b = quantised(x)
     back = np.ldexp(e4m3_values(codes), (b.astype(int) - 127)[:, None])
     assert np.all(np.abs(back - x) <= np.maximum(2.0 ** -4 * np.abs(x), np.ldexp(1.0, b.astype(int) - 137)[:, None]))
+
+
+def test_block_table_uploads_again_where_its_tensor_is_gone():
+    """A table first uploaded inside a scope is released with it; the next use uploads it anew."""
+    from tensor_cuda.backend import CudaBackend
+    from tensor_cuda.kv_cache import BlockTable
+
+    class Uploads(CudaBackend):
+        def from_host_sync(self, h):
+            return self.external(16, h.shape, h.dtype)
+
+    be = Uploads(NoDevice())
+    bt = BlockTable(be, 2, 8, 16, max_pages=4)
+    bt.reserve([5, 20])
+    inside = []
+    be.scope(lambda: inside.append(bt.device))
+    assert inside[0].disposed
+    again = bt.device
+    assert not again.disposed and again is not inside[0] and bt.device is again
+    bt.dispose()
