@@ -192,3 +192,23 @@ def test_vocabularies_beyond_the_sums_are_refused(be):
     with pytest.raises(F.MpcError, match="2\\^20 tokens") as e:
         be.sample(up(be, x, "f16"), u)
     assert e.value.status == F.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("t", [5.0, 10.0, 300.0])
+def test_flat_rows_cut_a_bin_again(be, t):
+    """Hot temperatures over a large vocabulary: a bin of T / 256 holds far more than 256 different logits, at the
+    borders of top_k and of top_p."""
+    x = np.random.default_rng(11).standard_normal((8, 50257))
+    for kw in (dict(k=5000, p=0.9), dict(k=5000), dict(p=0.9), dict(p=0.5, m=0.3), dict(k=40000, p=0.1), dict(k=50, p=0.9)):
+        check(be, x, "f32", uniform(8, int(t)), t=t, **kw)
+
+
+@pytest.mark.parametrize("rows,vocab", [(24, 3000), (400, 4099), (700, 20000), (5, 2048), (297, 2047)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_blocks_per_row(be, rows, vocab, dtype):
+    """Shapes that give a row one, two, four or eight blocks, each with every kind of setting."""
+    r = np.random.default_rng(rows)
+    x = r.standard_normal((rows, vocab)) * r.choice([0.01, 1.0, 4.0], (rows, 1))
+    check(be, x, dtype, uniform(rows, 1), r.choice([0.0, 0.7, 1.0, 20.0], rows), r.choice([0, 1, 40, 192, 500, 2000], rows),
+          r.choice([0.5, 0.95, 1.0], rows), r.choice([0.0, 0.0, 0.05, 0.6], rows))
+    check(be, x, dtype, uniform(rows, 2))
