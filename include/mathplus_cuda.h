@@ -379,7 +379,8 @@ int mpc_sdpa_paged(mpc_device *dev, const mpc_kv_desc *cache, const void *k_page
  * the most that a row may have), so the result does not depend on the order of the sum.
  * temperature <= 0 (or NaN), or min_p above 1: the largest logit, lowest index first. top_k <= 0, top_p >= 1 or NaN,
  * min_p <= 0 or NaN: off.
- * NaN logits count as -inf; a row with nothing above -inf gives token -1, prob 0, kept 0. u is clamped
+ * A token whose weight is under half a unit of the sums is kept and counted, but never drawn (by the exact sums only a
+ * u of 0 or next to 1 could). NaN logits count as -inf; a row with nothing above -inf gives token -1, prob 0, kept 0. u is clamped
  * to [0, 1) (NaN: 0). */
 typedef struct {
   int64_t rows, vocab, row_stride; /* logits element (r, i) at r * row_stride + i */

@@ -24,12 +24,12 @@
 // worst (a tail of weights just under half a unit): 2^-31 at 2^16 tokens, 2^-23, two steps of u next to 1, at 2^20.
 // Rows of more tokens are refused.
 //
-// A cluster of 1 to 8 CTAs takes a row, as many as keep the SMs busy. A few rows are bound by latency (cluster
-// barriers and remote reads), many by the instructions per token of the passes, the f64 exponentials (10 double
-// operations each) of the rows without top_k above all. Measured (GPU time of a replayed call): 4 rows of 50257 bf16 with
-// mixed settings 14.8 us (alike: greedy 6, top_k 50 15, top_p 0.9 26, top_k 1000 with top_p and min_p 45); 256 rows of
-// 131071 f32 with mixed settings 174 us (greedy 57, top_k 50 101, no filter 104, top_p 0.9 267); 134 MB at 6.55 TB/s
-// are 20.5 us.
+// A cluster of 1 to 8 CTAs takes a row. A few rows are bound by latency (cluster barriers and remote reads), many by the
+// passes over the row and their f64 exponentials (10 double operations each, at 33.5 M tokens a fifth of the time without
+// filters by the published rate; the rest is latency at 16 warps an SM). Measured (GPU time of a replayed call): 4 rows of
+// 50257 bf16 with mixed settings 14.7 us (alike: greedy 6, top_k 50 15, top_p 0.9 26, top_k 1000 with top_p and min_p 45);
+// 256 rows of 131071 f32 with mixed settings 173 us (greedy 57, top_k 50 102, no filter 104, top_p 0.9 265); 134 MB at
+// 6.55 TB/s are 20.5 us.
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
@@ -42,6 +42,9 @@ namespace mpc {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8;
+// kSmallK: top_k up to which the threads' maxima give the bound. Measured (by them / by the histogram) at top_k 1, 50, 100,
+// 192: 4 rows of 50257 bf16 12.2 / 13.9, 15.3 / 16.6, 17.7 / 17.7, 27.8 / 21.0 us; 256 of 131071 f32 87 / 113,
+// 102 / 130, 115 / 142, 167 / 159 us.
 constexpr int kBins = 8192, kList = kThreads, kSmallK = 192;
 constexpr float kBinsPerNat = 256.0f;
 
@@ -568,6 +571,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
       }
       __syncthreads();
       const bool need = outside && (by_p || gather);  // the weight of those above it
+      // Few enough to queue up. Measured (never / by the rule / always), 256 rows of 131071 f32: top_k 1000 211 / 171 / 162 us;
+      // top_p 0.9 over logits of spread 4 253 / 222 / 218, of spread 2 270 / 273 / 308, of spread 1 408 / 411 / 672.
       const bool few = outside < (unsigned)p.vocab / 16;
       if (lane == 0) sm.waiting[warp] = 0;
       __syncwarp();
@@ -943,9 +948,12 @@ int launch_cluster(mpc_device *dev, const SampleParams &p, int rows, cudaStream_
   return MPC_OK;
 }
 
-// CTAs per row: more than the two that an SM holds, so that the rows under way at a time stay in L2 for the later
-// passes (256 rows of 131071 f32: 2, 4 and 8 CTAs 186, 175 and 173 us; 4 rows of 50257 bf16: 19.1, 15.2 and 14.7 us),
-// and at least 1024 tokens each.
+// CTAs per row: up to 4 an SM and at least 1024 tokens each. More than the two that an SM holds, so that the rows under
+// way at a time stay in L2 for the later passes: 256 rows of 131071 f32 with mixed settings at 2, 4 and 8 CTAs a row 186,
+// 175 and 173 us, 4 rows of 50257 bf16 19.1, 15.2 and 14.7 us. Measured with bounds of 1, 4 and 16 an SM, top_p 0.9 and
+// top_k 50 alone: 300 x 131071 389, 305, 404 and 118, 101, 189 us; 300 x 50257 173, 163, 274 and 51, 57, 153 us. At 64 to
+// 148 rows the bound of 1 is ahead where all rows have the same setting: 148 x 50257 64, 142, 142 and 24, 80, 80 us; 64 x
+// 131071 67, 88, 87 and 25, 41, 41 us.
 template <int DT>
 int launch_sample(mpc_device *dev, const SampleParams &p, int rows, cudaStream_t st) {
   int c = 1;

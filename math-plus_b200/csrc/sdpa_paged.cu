@@ -2,8 +2,9 @@
 // form of mpc_sdpa (Backend.sdpa, packages/tensor-cpu/src/index.ts:821-840), Lq = 1.
 //
 // With s_j = scale * q.k_j for j < length: o = sum_j 2^(s'_j - m) v_j / sum_j 2^(s'_j - m), s' = s log2 e, m any
-// upper reference of s' (the running maximum). Every K/V row is read once and used for the query
-// heads that share it, so the cache's bytes bound the time and the work is split along the cache:
+// upper reference of s' (the running maximum). A K/V row is read once for each tile of the query heads that share
+// it: 16 on the tensor cores (8 at head dims above 128, or with f32 queries over 8 bits), 4 on the CUDA cores. With one
+// tile the cache's bytes bound the time, and the work is split along the cache:
 //
 // Split. An item is (sequence, K/V head, tile of its query heads); its keys are cut into tiles (16 or 32; more
 // where a table could hold 2^30 of them). The
@@ -19,11 +20,12 @@
 // CUDA-core kernel (f32 rows, and any head dim <= 256 or alignment): 8 lanes per key, 4 keys at a time, each
 // group of 8 lanes with its own running maximum, sum and O, which meet once per item.
 //
-// Measured (GPU time of a replayed call): 32 sequences of 500..8191 keys, 32 heads over 8 of 128, f16: 97.6 us, 5.8 TB/s
-// (a copy: 6.55), bound by HBM; 99999 and 131072 keys, 64 heads over 8 of 128, 8 bits: 108 us, 4.4 TB/s, bound by the
-// instructions that widen the codes; 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 26.1 us, 3.9 TB/s, bound by the
-// items' starts and joins; one of 1024 keys 10.5 us and, in f32 on the CUDA cores, 7 of 3..2050 keys with 10 heads over 5
-// of 80 / 72 22 us, both bound by latency.
+// Measured (GPU time of a replayed call): 32 sequences of 500..8191 keys, 32 heads over 8 of 128, f16: 98 us, 5.8 TB/s
+// (a copy: 6.55), bound by HBM; 99999 and 131072 keys, 64 heads over 8 of 128, 8 bits: 109 us, 4.4 TB/s, bound by the
+// instructions that widen the codes (f32 queries 115 us a call, f16 111); 64 sequences of 1..1024 keys, 12 heads of 64,
+// bf16: 25.5 us, 4.0 TB/s, bound by the items' starts and joins; one of 1024 keys 9.9 us and, in f32 on the CUDA cores, 7 of
+// 3..2050 keys with 10 heads over 5 of 80 / 72 22 us, both bound by latency. Wider groups than a tile: 8 x 8192 keys, 32
+// heads over 2 of 256, bf16, 71 us (two tiles; the bytes 20.5); in f32, four tiles, 843 us (41), with heads of 128 259 (20.5).
 #include <cfloat>
 
 #include "kv_cache.cuh"
@@ -34,9 +36,9 @@ namespace paged {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 4;  // resident on an SM, at most
-// Measured (3, 5, 8, 12 tiles an item): 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 23.5, 24.3, 25.2, 26.7 us; 32
-// sequences of 500..8191 keys, 8 heads of 128, f16: 100.8, 100.1, 98.5, 98.5 us; 2 of ~115k keys in 8 bits: 112, 111, 107,
-// 100 us. (0 against 8 with the joins left out: 35, 109 and 103 against 27, 98 and 91 us.)
+// Measured (3, 5, 8, 12 tiles an item): 64 sequences of 1..1024 keys, 12 heads of 64, bf16: 23.5, 24.2, 25.2, 26.4 us; 32
+// sequences of 500..8191 keys, 8 heads of 128, f16: 100.5, 100.2, 99.0, 98.5 us; 2 of ~115k keys in 8 bits: 113, 111, 108,
+// 100 us. (0 against 8 with the joins left out, of an earlier form: 35, 109 and 103 against 27, 98 and 91 us.)
 constexpr int kItemCost = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -555,7 +557,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const Params p) {
 // vote per tile in the common case, the row maximum by shuffles and a rescaling of O else. It is set 2^kHead
 // below the maximum so that small weights stay clear of f16's subnormals.
 // 8-bit rows: codes convert exactly to f16; Q is scaled by a power of two per row to [2^14, 2^15), where any
-// 16-bit q is exact in f16 down to 2^-28 of the row's largest (f32 q as two f16). K's scale multiplies the
+// 16-bit q is exact in f16 down to 2^-28 of the row's largest. An f32 q goes in as two f16, 22 of its 24 bits: the 2^-23
+// that is left is no more than the f32 sum of the products rounds. K's scale multiplies the
 // score. V's joins the weight: w = 2^(s' + e_v - M) with a reference M of its own, so that rows far below
 // the largest scale keep their precision.
 constexpr float kHead = 6.0f, kSlack = 14.0f;
@@ -638,9 +641,9 @@ __device__ __forceinline__ void key_pairs(const Chunk<KIND> &x, const Chunk<KIND
   }
 }
 
-// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value. TPI tiles of 16 keys at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks
-// per SM as the registers allow; over 8-bit rows of 128 two blocks of 32 keys a warp (94 us at 2 x ~115k keys, the join
-// left out) beat three of 16 (100 us).
+// DP: head dims padded to 64, 128 or 256; NT: tiles of 8 query heads; QS: numbers per query value. TPI tiles of 16 keys
+// at a time: 32 keys where their rows fit the registers that 16 longer ones take. Blocks per SM as the registers allow;
+// over 8-bit rows of 128 two blocks of 32 keys a warp (108 us at 2 x ~115k keys) beat three of 16 (118 us).
 template <int KIND, int DP>
 constexpr int tiles_at_once() { return DP == 64 || (DP == 128 && KIND == kE4M3) ? 2 : 1; }
 constexpr int blocks_per_sm(bool e4m3, int dp, int heads) { return dp == 256 || heads == 16 || (dp == 128 && e4m3) ? 2 : 3; }
@@ -969,7 +972,8 @@ static int plan_of(mpc_device *dev, const mpc_kv_desc *c, const mpc_sdpa_paged_d
     if (pl->tile >= (1 << 30)) return fail(MPC_ERR_UNSUPPORTED, "mpc_sdpa_paged: too many sequences and heads");
     pl->tile *= 2;
   }
-  // As many CTAs as are resident, fewer where even the longest lengths give fewer tiles than warps.
+  // CTAs: as many as are resident on the tensor cores, three an SM on the CUDA cores (their registers, 118 to 254 a
+  // thread, would let two to four be resident); fewer where even the longest lengths give fewer tiles than warps.
   const long long per = (d->max_pages * c->page_size + kWarps * pl->tile - 1) / (kWarps * pl->tile);
   const long long sms = (long long)dev->prop.multiProcessorCount * (tc ? blocks_per_sm(c->dtype == MPC_E4M3, pl->dp, pl->gt) : 3);
   const long long heads = c->hk * pl->qt;
